@@ -1,0 +1,340 @@
+"""A model's input layers: what a trainer does with node ids and gathered rows
+before its first layer (no reference counterpart; there it is torch code of the
+training scripts).
+
+* ``embedding`` / ``NodeEmbedding``: rows of a learnable table, times a scale,
+  for node types without stored features (or tokens), with the gradient by
+  sorted ids: dense, or as the distinct rows for tables too large for that.
+* ``layer_norm`` / ``LayerNorm``: layer norm of gathered rows, forward and
+  backward.
+
+``GIDS.GIDS(node_embeddings=..., feature_norm=...)`` applies them to the batches
+it hands out. All run as hand-written kernels in the library behind
+``BAM_Feature_Store`` (imported on first use) on the current stream, take
+float32, float16 and bfloat16 CUDA tensors, sum in float32 and repeat bit for
+bit. Workspaces come from torch's allocator for each call, so calls on several
+streams and in several captured graphs share nothing.
+
+An id outside its table gives a zero row and no gradient, and raises at the next
+embedding call on that device, or at ``check_ids``. A backward pass that is
+captured into a CUDA graph must not meet an eager graph of the same parameters
+that is still alive (torch's rule for every op): drop eager losses and outputs first.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .sampler import _store_module
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _type(t: torch.dtype, what: str) -> int:
+    if t not in _TYPES:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t}")
+    return _TYPES[t]
+
+
+def _need_cuda(device: torch.device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if device.type != "cuda":
+        raise ValueError(f"CUDA tensors expected, not {device}")
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _check_ids(ids: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be int32 or int64, not {ids.dtype}")
+    return ids.contiguous()
+
+
+def _as_rows(t: torch.Tensor, dim: int) -> torch.Tensor:
+    """t as a matrix of rows [*, dim] whose columns are consecutive (a view where there is one)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
+    if (dim > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+        t = t.contiguous()
+    return t
+
+
+def _padding(padding_idx, num_rows: int) -> int:
+    if padding_idx is None:
+        return -1
+    p = int(padding_idx)
+    if not -num_rows <= p < num_rows:
+        raise ValueError(f"padding_idx {p} is outside the table of {num_rows} rows")
+    return p + num_rows if p < 0 else p
+
+
+def check_ids(device=None):
+    """Wait for the current stream of ``device`` and raise RuntimeError if an
+    embedding call there met an id outside its table since the last check."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
+    _store_module().embedding_check(device.index, _stream(device))
+
+
+# ------------------------------------------------------------------ embedding
+def _embedding_forward(ids, weight, scale, dtype):
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be a matrix, not {tuple(weight.shape)}")
+    num_rows, dim = weight.shape
+    wt, ot = _type(weight.dtype, "weight"), _type(dtype, "dtype")
+    _need_cuda(weight.device, ids=ids, weight=weight)
+    if dim > 1 and weight.stride(1) != 1:
+        raise ValueError("the columns of weight must be consecutive (stride 1)")
+    ids = _check_ids(ids)
+    out = torch.empty((*ids.shape, dim), dtype=dtype, device=weight.device)
+    if dim:
+        _store_module().embedding(weight.device.index, out.data_ptr(), ot, dim, weight.data_ptr(), wt,
+                                  weight.stride(0), num_rows, dim, ids.data_ptr(), ids.element_size(), ids.numel(),
+                                  scale, _stream(weight.device))
+    return out
+
+
+def _grad_args(ids, grad, num_rows, dtype):
+    ids = _check_ids(ids)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
+        raise ValueError(f"grad {tuple(grad.shape)} does not hold one row for each of the ids {tuple(ids.shape)}")
+    dim = grad.shape[-1]
+    if dim < 1:
+        raise ValueError("grad has no columns")
+    dtype = grad.dtype if dtype is None else dtype
+    gt, wt = _type(grad.dtype, "grad"), _type(dtype, "dtype")
+    _need_cuda(grad.device, ids=ids, grad=grad)
+    rows = _as_rows(grad, dim)
+    ws = torch.empty(_store_module().embedding_grad_workspace(ids.numel(), num_rows, dim), dtype=torch.uint8,
+                     device=grad.device)
+    return ids, rows, dim, dtype, gt, wt, ws
+
+
+def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None):
+    """The gradient of ``embedding`` as a dense table [num_rows, dim]: row v is
+    ``scale`` times the sum of the rows of ``grad`` whose id is v (in position
+    order, in float32), rounded to ``dtype`` (grad's by default, or float32).
+    Ids equal to ``padding_idx`` are left out."""
+    num_rows = int(num_rows)
+    pad = _padding(padding_idx, num_rows)
+    ids, g, dim, dtype, gt, wt, ws = _grad_args(ids, grad, num_rows, dtype)
+    dw = torch.empty((num_rows, dim), dtype=dtype, device=grad.device)
+    _store_module().embedding_grad(grad.device.index, dw.data_ptr(), wt, dim, num_rows, dim, g.data_ptr(), gt,
+                                   g.stride(0), ids.data_ptr(), ids.element_size(), ids.numel(), pad, scale,
+                                   ws.data_ptr(), ws.numel(), _stream(grad.device))
+    return dw
+
+
+def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None):
+    """The gradient of ``embedding`` as its distinct rows: ``(rows, values)``,
+    the ids that occur (ascending, int64; without ``padding_idx``) and for each
+    the row ``embedding_grad`` would hold. Waits for the stream once, for the
+    number of rows, so it cannot be captured into a graph."""
+    num_rows = int(num_rows)
+    pad = _padding(padding_idx, num_rows)
+    ids, g, dim, dtype, gt, wt, ws = _grad_args(ids, grad, num_rows, dtype)
+    m, dev, stream = _store_module(), grad.device, _stream(grad.device)
+    n = ids.numel()
+    count = m.embedding_group(dev.index, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
+                              ws.numel(), 0, stream)
+    rows = torch.empty(count, dtype=torch.int64, device=dev)
+    values = torch.empty((count, dim), dtype=dtype, device=dev)
+    m.embedding_grad_rows(dev.index, rows.data_ptr(), values.data_ptr(), wt, dim, count, num_rows, dim, g.data_ptr(),
+                          gt, g.stride(0), n, scale, ws.data_ptr(), ws.numel(), stream)
+    return rows, values
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx, sparse, dtype):
+        ctx.save_for_backward(ids)
+        ctx.conf = (weight.shape[0], scale, padding_idx, sparse, weight.dtype)
+        return _embedding_forward(ids, weight, scale, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        num_rows, scale, padding_idx, sparse, dtype = ctx.conf
+        if not sparse:
+            dw = embedding_grad(ids, grad, num_rows, scale, padding_idx, dtype)
+        else:
+            rows, values = embedding_grad_rows(ids, grad, num_rows, scale, padding_idx, dtype)
+            dw = torch.sparse_coo_tensor(rows.unsqueeze(0), values, (num_rows, grad.shape[-1]), is_coalesced=True)
+        return None, dw, None, None, None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None, sparse=False, dtype=None):
+    """``scale * weight[ids]`` as a tensor [*ids.shape, dim] of ``dtype`` (the
+    table's; any of the three types if the table is float32). Differentiable in
+    ``weight``: rows of ``padding_idx`` get no gradient, and with ``sparse`` the
+    gradient is a coalesced sparse tensor of the distinct rows (for
+    torch.optim.SparseAdam and the like) instead of a dense table."""
+    dtype = weight.dtype if dtype is None else dtype
+    scale = float(scale)
+    if padding_idx is not None:
+        padding_idx = _padding(padding_idx, weight.shape[0])
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(ids, weight, scale, padding_idx, bool(sparse), dtype)
+    return _embedding_forward(ids, weight, scale, dtype)
+
+
+class NodeEmbedding(torch.nn.Module):
+    """A learnable table of ``num_rows`` rows, looked up by id (``embedding``).
+
+    ``padding_idx`` starts as a zero row and gets no gradient; ``sparse`` gives
+    the gradient as its distinct rows; ``out_dtype`` is the type of the looked
+    up rows (a float32 table can feed a 16-bit model)."""
+
+    def __init__(self, num_rows, dim, scale=1.0, padding_idx=None, sparse=False, dtype=torch.float32, out_dtype=None,
+                 device=None):
+        super().__init__()
+        self.num_rows, self.dim = int(num_rows), int(dim)
+        self.scale = float(scale)
+        self.padding_idx = None if padding_idx is None else _padding(padding_idx, self.num_rows)
+        self.sparse = bool(sparse)
+        self.out_dtype = out_dtype
+        self.weight = torch.nn.Parameter(torch.empty((self.num_rows, self.dim), dtype=dtype, device=device))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            self.weight.normal_(0.0, 1.0 / math.sqrt(self.dim))
+            if self.padding_idx is not None:
+                self.weight[self.padding_idx].zero_()
+
+    def forward(self, ids):
+        return embedding(ids, self.weight, self.scale, self.padding_idx, self.sparse, self.out_dtype)
+
+    def extra_repr(self):
+        return f"{self.num_rows}, {self.dim}, scale={self.scale}, padding_idx={self.padding_idx}, sparse={self.sparse}"
+
+
+# ----------------------------------------------------------------- layer norm
+def _params(x, weight, bias):
+    """dim and the type code of weight and bias (x's where there are none)."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have rows of at least one column, not {tuple(x.shape)}")
+    dim = x.shape[-1]
+    xt = _type(x.dtype, "x")
+    pt = None
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.shape != (dim,):
+            raise ValueError(f"{name} must have shape ({dim},), not {tuple(p.shape)}")
+        if dim > 1 and p.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+        t = _type(p.dtype, name)
+        if pt is not None and t != pt:
+            raise ValueError("weight and bias must have one type")
+        pt = t
+    if pt is None:
+        pt = xt
+    if pt not in (xt, 0):
+        raise ValueError("weight and bias must have x's type or float32")
+    return dim, xt, pt
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _layer_norm_forward(x, weight, bias, eps, stats):
+    dim, xt, pt = _params(x, weight, bias)
+    _need_cuda(x.device, x=x, weight=weight, bias=bias)
+    rows = _as_rows(x, dim)
+    n = rows.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean = torch.empty(n, dtype=torch.float32, device=x.device)
+        rstd = torch.empty(n, dtype=torch.float32, device=x.device)
+    _store_module().layer_norm(x.device.index, y.data_ptr(), dim, _ptr(mean), _ptr(rstd), rows.data_ptr(), xt,
+                               rows.stride(0), _ptr(weight), _ptr(bias), pt, n, dim, eps, _stream(x.device))
+    return y, mean, rstd
+
+
+def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), param_dtype=None):
+    """``(dx, dweight, dbias)`` of ``layer_norm`` from the gradient of its
+    output and the mean and rstd of every row (float32, as
+    ``layer_norm_stats`` returns them). ``need`` says which are wanted (None for
+    the others). dweight and dbias have weight's type; without a weight,
+    ``param_dtype`` (x's by default, or float32)."""
+    dim, xt, pt = _params(x, weight, None)
+    ptype = weight.dtype if weight is not None else param_dtype or x.dtype
+    if weight is None:
+        if ptype not in (x.dtype, torch.float32):
+            raise ValueError("param_dtype must be x's type or float32")
+        pt = _TYPES[ptype]
+    if grad.shape != x.shape or grad.dtype != x.dtype:
+        raise ValueError(f"grad must be like x: {tuple(x.shape)} {x.dtype}, not {tuple(grad.shape)} {grad.dtype}")
+    _need_cuda(x.device, x=x, grad=grad, mean=mean, rstd=rstd, weight=weight)
+    xr, gr = _as_rows(x, dim), _as_rows(grad, dim)
+    n = xr.shape[0]
+    for name, s in (("mean", mean), ("rstd", rstd)):
+        if s.dtype != torch.float32 or s.numel() != n or not s.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 tensor of {n} elements")
+    m = _store_module()
+    want_p = need[1] or need[2]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    dw = torch.empty(dim, dtype=ptype, device=x.device) if need[1] else None
+    db = torch.empty(dim, dtype=ptype, device=x.device) if need[2] else None
+    ws = torch.empty(m.layer_norm_grad_workspace(n, dim) if want_p else 0, dtype=torch.uint8, device=x.device)
+    m.layer_norm_grad(x.device.index, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
+                      gr.stride(0), xr.data_ptr(), xt, xr.stride(0), _ptr(weight), pt, mean.data_ptr(),
+                      rstd.data_ptr(), n, dim, ws.data_ptr(), ws.numel(), _stream(x.device))
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _layer_norm_forward(x, weight, bias, eps, True)
+        ctx.bias_type = None if bias is None else bias.dtype
+        ctx.save_for_backward(x, mean, rstd, weight)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, mean, rstd, weight = ctx.saved_tensors
+        return *layer_norm_grad(grad, x, mean, rstd, weight, ctx.needs_input_grad[:3], ctx.bias_type), None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last dimension of ``x``: ``(x - mean) / sqrt(var +
+    eps) * weight + bias`` in x's type; weight and bias [dim] are of x's type or
+    float32, or None. Differentiable in all three."""
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _layer_norm_forward(x, weight, bias, float(eps), False)[0]
+
+
+def layer_norm_stats(x, weight=None, bias=None, eps=1e-5):
+    """``(y, mean, rstd)``: ``layer_norm`` (without autograd) and the float32
+    statistics of every row that ``layer_norm_grad`` takes."""
+    return _layer_norm_forward(x, weight, bias, float(eps), True)
+
+
+class LayerNorm(torch.nn.Module):
+    """``layer_norm`` with learnable weight and bias (``affine``; ``bias=False`` leaves the bias out)."""
+
+    def __init__(self, dim, eps=1e-5, affine=True, bias=True, dtype=torch.float32, device=None):
+        super().__init__()
+        self.dim, self.eps = int(dim), float(eps)
+        self.weight = torch.nn.Parameter(torch.ones(self.dim, dtype=dtype, device=device)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(self.dim, dtype=dtype, device=device)) if affine and bias else None
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return f"{self.dim}, eps={self.eps}, affine={self.weight is not None}"

@@ -26,9 +26,10 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-CU_SOURCES = ["gather.cu", "store.cu", "noalloc.cu", "sampler.cu"]
+CU_SOURCES = ["gather.cu", "store.cu", "noalloc.cu", "sampler.cu", "embedding.cu", "layer_norm.cu"]
 CPP_SOURCES = ["backing.cpp", "abi.cpp"]
-HEADERS = [os.path.join(CSRC, "gids_internal.hpp"), os.path.join(INCLUDE, "gids_b200.h")]
+HEADERS = [os.path.join(CSRC, "gids_internal.hpp"), os.path.join(CSRC, "layers.hpp"), os.path.join(CSRC, "rows.cuh"),
+           os.path.join(INCLUDE, "gids_b200.h")]
 
 
 def _pymod_path() -> str:

@@ -9,6 +9,7 @@
 #include <string>
 
 #include "gids_internal.hpp"
+#include "layers.hpp"
 
 struct gids_ctrls {
   gids::Controllers c;
@@ -560,6 +561,84 @@ int gids_out_degree(int device, const void* indices, int index_bytes, uint64_t n
                     uint32_t* counts, void* stream) {
   return guarded([&] {
     gids::out_degree(device, indices, index_bytes, num_edges, num_nodes, counts, (cudaStream_t)stream);
+  });
+}
+
+int gids_embedding(int device, void* out, int out_type, int64_t out_stride, const void* weight, int weight_type,
+                   int64_t weight_stride, int64_t num_rows, int64_t dim, const void* ids, int id_bytes, int64_t n,
+                   float scale, void* stream) {
+  return guarded([&] {
+    gids::embedding(device, {out, out_type, out_stride}, {const_cast<void*>(weight), weight_type, weight_stride},
+                    num_rows, dim, ids, id_bytes, n, scale, (cudaStream_t)stream);
+  });
+}
+
+int gids_embedding_check(int device, void* stream) {
+  return guarded([&] { gids::embedding_check(device, (cudaStream_t)stream); });
+}
+
+int gids_embedding_grad_workspace(int64_t n, int64_t num_rows, int64_t dim, uint64_t* bytes) {
+  return guarded([&] {
+    NEED(bytes);
+    *bytes = gids::embedding_grad_workspace(n, num_rows, dim);
+  });
+}
+
+int gids_embedding_grad(int device, void* dweight, int weight_type, int64_t dweight_stride, int64_t num_rows,
+                        int64_t dim, const void* grad, int grad_type, int64_t grad_stride, const void* ids,
+                        int id_bytes, int64_t n, int64_t padding_idx, float scale, void* workspace,
+                        uint64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    gids::embedding_grad(device, {dweight, weight_type, dweight_stride}, num_rows, dim,
+                         {const_cast<void*>(grad), grad_type, grad_stride}, ids, id_bytes, n, padding_idx, scale,
+                         workspace, workspace_bytes, (cudaStream_t)stream);
+  });
+}
+
+int gids_embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
+                         int64_t dim, void* workspace, uint64_t workspace_bytes, uint64_t* count_dev,
+                         uint64_t* count_host, void* stream) {
+  return guarded([&] {
+    gids::embedding_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, workspace, workspace_bytes, count_dev,
+                          count_host, (cudaStream_t)stream);
+  });
+}
+
+int gids_embedding_grad_rows(int device, int64_t* rows, void* values, int value_type, int64_t values_stride,
+                             int64_t capacity, int64_t num_rows, int64_t dim, const void* grad, int grad_type,
+                             int64_t grad_stride, int64_t n, float scale, void* workspace, uint64_t workspace_bytes,
+                             void* stream) {
+  return guarded([&] {
+    gids::embedding_grad_rows(device, rows, {values, value_type, values_stride}, capacity, num_rows, dim,
+                              {const_cast<void*>(grad), grad_type, grad_stride}, n, scale, workspace, workspace_bytes,
+                              (cudaStream_t)stream);
+  });
+}
+
+int gids_layer_norm(int device, void* y, int64_t y_stride, float* mean, float* rstd, const void* x, int x_type,
+                    int64_t x_stride, const void* weight, const void* bias, int param_type, int64_t n, int64_t dim,
+                    float eps, void* stream) {
+  return guarded([&] {
+    gids::layer_norm(device, {y, x_type, y_stride}, mean, rstd, {const_cast<void*>(x), x_type, x_stride}, weight, bias,
+                     param_type, n, dim, eps, (cudaStream_t)stream);
+  });
+}
+
+int gids_layer_norm_grad_workspace(int64_t n, int64_t dim, uint64_t* bytes) {
+  return guarded([&] {
+    NEED(bytes);
+    *bytes = gids::layer_norm_grad_workspace(n, dim);
+  });
+}
+
+int gids_layer_norm_grad(int device, void* dx, int64_t dx_stride, void* dweight, void* dbias, const void* grad,
+                         int64_t grad_stride, const void* x, int x_type, int64_t x_stride, const void* weight,
+                         int param_type, const float* mean, const float* rstd, int64_t n, int64_t dim, void* workspace,
+                         uint64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    gids::layer_norm_grad(device, {dx, x_type, dx_stride}, dweight, dbias,
+                          {const_cast<void*>(grad), x_type, grad_stride}, {const_cast<void*>(x), x_type, x_stride},
+                          mean, rstd, weight, param_type, n, dim, workspace, workspace_bytes, (cudaStream_t)stream);
   });
 }
 

@@ -463,6 +463,103 @@ PYBIND11_MODULE(BAM_Feature_Store, m) {
       py::arg("device"), py::arg("indptr"), py::arg("indices"), py::arg("index_bytes"), py::arg("num_nodes"),
       py::arg("iters"), py::arg("damping"), py::arg("pv"), py::arg("keys") = 0, py::arg("stream") = 0,
       py::call_guard<py::gil_scoped_release>());
+  // extension: a model's input layers (gids_embedding*, gids_layer_norm*)
+  m.def(
+      "embedding",
+      [](int device, uint64_t out, int out_type, int64_t out_stride, uint64_t weight, int weight_type,
+         int64_t weight_stride, int64_t num_rows, int64_t dim, uint64_t ids, int id_bytes, int64_t n, float scale,
+         uint64_t stream) {
+        check(gids_embedding(device, (void*)out, out_type, out_stride, (const void*)weight, weight_type, weight_stride,
+                             num_rows, dim, (const void*)ids, id_bytes, n, scale, (void*)stream));
+      },
+      py::arg("device"), py::arg("out"), py::arg("out_type"), py::arg("out_stride"), py::arg("weight"),
+      py::arg("weight_type"), py::arg("weight_stride"), py::arg("num_rows"), py::arg("dim"), py::arg("ids"),
+      py::arg("id_bytes"), py::arg("n"), py::arg("scale") = 1.0f, py::arg("stream") = 0,
+      py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "embedding_check", [](int device, uint64_t stream) { check(gids_embedding_check(device, (void*)stream)); },
+      py::arg("device"), py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "embedding_grad_workspace",
+      [](int64_t n, int64_t num_rows, int64_t dim) {
+        uint64_t b = 0;
+        check(gids_embedding_grad_workspace(n, num_rows, dim, &b));
+        return b;
+      },
+      py::arg("n"), py::arg("num_rows"), py::arg("dim"));
+  m.def(
+      "embedding_grad",
+      [](int device, uint64_t dweight, int weight_type, int64_t dweight_stride, int64_t num_rows, int64_t dim,
+         uint64_t grad, int grad_type, int64_t grad_stride, uint64_t ids, int id_bytes, int64_t n, int64_t padding_idx,
+         float scale, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream) {
+        check(gids_embedding_grad(device, (void*)dweight, weight_type, dweight_stride, num_rows, dim,
+                                  (const void*)grad, grad_type, grad_stride, (const void*)ids, id_bytes, n, padding_idx,
+                                  scale, (void*)workspace, workspace_bytes, (void*)stream));
+      },
+      py::arg("device"), py::arg("dweight"), py::arg("weight_type"), py::arg("dweight_stride"), py::arg("num_rows"),
+      py::arg("dim"), py::arg("grad"), py::arg("grad_type"), py::arg("grad_stride"), py::arg("ids"),
+      py::arg("id_bytes"), py::arg("n"), py::arg("padding_idx") = -1, py::arg("scale") = 1.0f,
+      py::arg("workspace") = 0, py::arg("workspace_bytes") = 0, py::arg("stream") = 0,
+      py::call_guard<py::gil_scoped_release>());
+  // returns the number of distinct rows (waits for the stream) unless count_dev is given
+  m.def(
+      "embedding_group",
+      [](int device, uint64_t ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx, int64_t dim,
+         uint64_t workspace, uint64_t workspace_bytes, uint64_t count_dev, uint64_t stream) {
+        uint64_t host = 0;
+        check(gids_embedding_group(device, (const void*)ids, id_bytes, n, num_rows, padding_idx, dim, (void*)workspace,
+                                   workspace_bytes, (uint64_t*)count_dev, count_dev ? nullptr : &host, (void*)stream));
+        return host;
+      },
+      py::arg("device"), py::arg("ids"), py::arg("id_bytes"), py::arg("n"), py::arg("num_rows"),
+      py::arg("padding_idx"), py::arg("dim"), py::arg("workspace"), py::arg("workspace_bytes"),
+      py::arg("count_dev") = 0, py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "embedding_grad_rows",
+      [](int device, uint64_t rows, uint64_t values, int value_type, int64_t values_stride, int64_t capacity,
+         int64_t num_rows, int64_t dim, uint64_t grad, int grad_type, int64_t grad_stride, int64_t n, float scale,
+         uint64_t workspace, uint64_t workspace_bytes, uint64_t stream) {
+        check(gids_embedding_grad_rows(device, (int64_t*)rows, (void*)values, value_type, values_stride, capacity,
+                                       num_rows, dim, (const void*)grad, grad_type, grad_stride, n, scale,
+                                       (void*)workspace, workspace_bytes, (void*)stream));
+      },
+      py::arg("device"), py::arg("rows"), py::arg("values"), py::arg("value_type"), py::arg("values_stride"),
+      py::arg("capacity"), py::arg("num_rows"), py::arg("dim"), py::arg("grad"), py::arg("grad_type"),
+      py::arg("grad_stride"), py::arg("n"), py::arg("scale"), py::arg("workspace"), py::arg("workspace_bytes"),
+      py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "layer_norm",
+      [](int device, uint64_t y, int64_t y_stride, uint64_t mean, uint64_t rstd, uint64_t x, int x_type,
+         int64_t x_stride, uint64_t weight, uint64_t bias, int param_type, int64_t n, int64_t dim, float eps,
+         uint64_t stream) {
+        check(gids_layer_norm(device, (void*)y, y_stride, (float*)mean, (float*)rstd, (const void*)x, x_type, x_stride,
+                              (const void*)weight, (const void*)bias, param_type, n, dim, eps, (void*)stream));
+      },
+      py::arg("device"), py::arg("y"), py::arg("y_stride"), py::arg("mean"), py::arg("rstd"), py::arg("x"),
+      py::arg("x_type"), py::arg("x_stride"), py::arg("weight"), py::arg("bias"), py::arg("param_type"), py::arg("n"),
+      py::arg("dim"), py::arg("eps"), py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "layer_norm_grad_workspace",
+      [](int64_t n, int64_t dim) {
+        uint64_t b = 0;
+        check(gids_layer_norm_grad_workspace(n, dim, &b));
+        return b;
+      },
+      py::arg("n"), py::arg("dim"));
+  m.def(
+      "layer_norm_grad",
+      [](int device, uint64_t dx, int64_t dx_stride, uint64_t dweight, uint64_t dbias, uint64_t grad,
+         int64_t grad_stride, uint64_t x, int x_type, int64_t x_stride, uint64_t weight, int param_type, uint64_t mean,
+         uint64_t rstd, int64_t n, int64_t dim, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream) {
+        check(gids_layer_norm_grad(device, (void*)dx, dx_stride, (void*)dweight, (void*)dbias, (const void*)grad,
+                                   grad_stride, (const void*)x, x_type, x_stride, (const void*)weight, param_type,
+                                   (const float*)mean, (const float*)rstd, n, dim, (void*)workspace, workspace_bytes,
+                                   (void*)stream));
+      },
+      py::arg("device"), py::arg("dx"), py::arg("dx_stride"), py::arg("dweight"), py::arg("dbias"), py::arg("grad"),
+      py::arg("grad_stride"), py::arg("x"), py::arg("x_type"), py::arg("x_stride"), py::arg("weight"),
+      py::arg("param_type"), py::arg("mean"), py::arg("rstd"), py::arg("n"), py::arg("dim"), py::arg("workspace"),
+      py::arg("workspace_bytes"), py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
   // extension: one process driving every GPU of a sharded cache
   m.def("share_shards", [](py::list stores) {
     std::vector<gids_store_t*> v;

@@ -1,0 +1,121 @@
+// Device helpers of the row kernels (embedding.cu, layer_norm.cu): element
+// types, vector loads and stores of rows, and a division by a launch constant.
+// Arithmetic is float32 throughout; a value is rounded to its type once, when
+// it is stored (round to nearest even).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace gids {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// VEC consecutive elements, moved in pieces of at most 16 bytes; the address
+// is aligned to min(16, sizeof(T) * VEC).
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) RowVec {
+  T v[VEC];
+};
+
+template <int BYTES>
+struct Piece;
+template <>
+struct Piece<2> {
+  using type = unsigned short;
+};
+template <>
+struct Piece<4> {
+  using type = unsigned int;
+};
+template <>
+struct Piece<8> {
+  using type = uint2;
+};
+template <>
+struct Piece<16> {
+  using type = uint4;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ RowVec<T, VEC> load_vec(const T* p) {
+  constexpr int B = sizeof(T) * VEC < 16 ? (int)sizeof(T) * VEC : 16;
+  using P = typename Piece<B>::type;
+  constexpr int N = (int)sizeof(T) * VEC / B;
+  RowVec<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < N; i++) reinterpret_cast<P*>(&r)[i] = __ldg(reinterpret_cast<const P*>(p) + i);
+  return r;
+}
+
+// The same for rows that are read once, and that the kernel may overwrite
+// (a coherent load, which evicts first).
+template <typename T, int VEC>
+__device__ __forceinline__ RowVec<T, VEC> load_row(const T* p) {
+  constexpr int B = sizeof(T) * VEC < 16 ? (int)sizeof(T) * VEC : 16;
+  using P = typename Piece<B>::type;
+  constexpr int N = (int)sizeof(T) * VEC / B;
+  RowVec<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < N; i++) reinterpret_cast<P*>(&r)[i] = __ldcs(reinterpret_cast<const P*>(p) + i);
+  return r;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_raw(T* p, const RowVec<T, VEC>& r) {
+  constexpr int B = sizeof(T) * VEC < 16 ? (int)sizeof(T) * VEC : 16;
+  using P = typename Piece<B>::type;
+  constexpr int N = (int)sizeof(T) * VEC / B;
+#pragma unroll
+  for (int i = 0; i < N; i++) reinterpret_cast<P*>(p)[i] = reinterpret_cast<const P*>(&r)[i];
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
+  RowVec<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; i++) r.v[i] = from_f32<T>(v[i]);
+  store_raw(p, r);
+}
+
+// n / d for 32-bit n by a multiplication (d >= 1 fixed at launch): with
+// l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
+// n / d = (t + ((n - t) >> min(l, 1))) >> max(l - 1, 0), t = mulhi(m, n)
+// (Granlund and Montgomery, "Division by invariant integers using
+// multiplication", PLDI 1994).
+struct FastDiv {
+  unsigned int d = 1, m = 1, s1 = 0, s2 = 0;
+  FastDiv() = default;
+  explicit FastDiv(unsigned int div) : d(div) {
+    unsigned int l = 0;
+    while (l < 32 && (1ull << l) < div) l++;
+    m = (unsigned int)((((1ull << l) - div) << 32) / div + 1ull);
+    s1 = l < 1 ? l : 1;
+    s2 = l < 1 ? 0 : l - 1;
+  }
+  __device__ __forceinline__ unsigned int div(unsigned int n) const {
+    const unsigned int t = __umulhi(m, n);
+    return (t + ((n - t) >> s1)) >> s2;
+  }
+};
+
+}  // namespace gids

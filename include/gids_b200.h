@@ -432,6 +432,81 @@ GIDS_API int gids_pagerank(int device, const int64_t *indptr, const void *indice
 GIDS_API int gids_out_degree(int device, const void *indices, int index_bytes, uint64_t num_edges, uint64_t num_nodes,
                              uint32_t *counts, void *stream);
 
+/* -------------------------------------------------- a model's input layers --
+ * What a trainer does with node ids and gathered rows before its first layer;
+ * no reference counterpart (there it is DGL / torch code of the training
+ * scripts). Rows are row-major matrices in device memory: `stride` elements
+ * from row to row (a stride of 0 repeats one row where a matrix is read), the
+ * columns of a row consecutive, no alignment beyond the element's. Element
+ * types are GIDS_F32, GIDS_F16 and GIDS_BF16. Sums and statistics are float32;
+ * every result is rounded to its type once. Nothing is summed with atomics:
+ * the same call gives the same bits. All calls run on `stream` of `device`,
+ * allocate no device memory, and, count_host apart, wait for nothing and can be
+ * captured into a graph. A workspace (256-byte aligned device memory) belongs
+ * to one call at a time. */
+#define GIDS_F32 0
+#define GIDS_F16 1
+#define GIDS_BF16 2
+
+/* out[i, :] = scale * weight[ids[i], :], i < n, `dim` columns of a table of
+ * num_rows rows. ids: int32 or int64 (id_bytes 4 or 8). out has the table's
+ * type, or any type if the table is float32; in the table's type a scale of 1
+ * copies the bits. An id outside the table gives a
+ * zero row; the next embedding call on the device (before it does anything), or
+ * gids_embedding_check, returns GIDS_E_RANGE for it once. */
+GIDS_API int gids_embedding(int device, void *out, int out_type, int64_t out_stride, const void *weight,
+                            int weight_type, int64_t weight_stride, int64_t num_rows, int64_t dim, const void *ids,
+                            int id_bytes, int64_t n, float scale, void *stream);
+/* Waits for `stream` and reports ids outside their table (GIDS_E_RANGE). */
+GIDS_API int gids_embedding_check(int device, void *stream);
+
+/* The gradient of gids_embedding by sorted ids. dweight[v, :] = scale * the sum
+ * of grad[i, :] over the i with ids[i] = v, in position order; rows without an
+ * id are zero. Positions whose id is padding_idx (-1: none) or lies outside
+ * the table are left out (the latter are reported as above). dweight has the
+ * gradient's type or is float32. gids_embedding_grad_workspace: bytes of
+ * workspace for this and the two calls below. */
+GIDS_API int gids_embedding_grad_workspace(int64_t n, int64_t num_rows, int64_t dim, uint64_t *bytes);
+GIDS_API int gids_embedding_grad(int device, void *dweight, int weight_type, int64_t dweight_stride, int64_t num_rows,
+                                 int64_t dim, const void *grad, int grad_type, int64_t grad_stride, const void *ids,
+                                 int id_bytes, int64_t n, int64_t padding_idx, float scale, void *workspace,
+                                 uint64_t workspace_bytes, void *stream);
+/* The same gradient as the distinct rows, for tables too large for a dense
+ * one, in two calls. gids_embedding_group sorts the ids into the workspace and
+ * counts the distinct ones that are neither padding nor outside the table:
+ * count_dev (device, may be NULL) receives the number without a wait;
+ * count_host (may be NULL) makes the call wait and return it there (refused
+ * with GIDS_E_STATE on a stream that is being captured).
+ * gids_embedding_grad_rows, with the same n, num_rows, dim and workspace,
+ * then writes them in ascending order to rows[k] and their summed gradients to
+ * values[k, :], k < min(number, capacity). */
+GIDS_API int gids_embedding_group(int device, const void *ids, int id_bytes, int64_t n, int64_t num_rows,
+                                  int64_t padding_idx, int64_t dim, void *workspace, uint64_t workspace_bytes,
+                                  uint64_t *count_dev, uint64_t *count_host, void *stream);
+GIDS_API int gids_embedding_grad_rows(int device, int64_t *rows, void *values, int value_type, int64_t values_stride,
+                                      int64_t capacity, int64_t num_rows, int64_t dim, const void *grad, int grad_type,
+                                      int64_t grad_stride, int64_t n, float scale, void *workspace,
+                                      uint64_t workspace_bytes, void *stream);
+
+/* y[i, :] = (x[i, :] - m) r * weight + bias with m the mean and r = 1 /
+ * sqrt(v + eps), v the mean squared difference from m, of row i. weight and
+ * bias (dim elements of param_type, which is x's type or GIDS_F32) may be NULL
+ * (1 and 0). mean and rstd (n float32 each, both or neither NULL) receive m
+ * and r for the gradient. y may be x (same address and stride). */
+GIDS_API int gids_layer_norm(int device, void *y, int64_t y_stride, float *mean, float *rstd, const void *x,
+                             int x_type, int64_t x_stride, const void *weight, const void *bias, int param_type,
+                             int64_t n, int64_t dim, float eps, void *stream);
+/* The gradients of gids_layer_norm from the gradient of y (of x's type) and the
+ * mean and rstd it stored: dx (x's type), dweight = the sum of grad * xh and
+ * dbias = the sum of grad over the rows (param_type), xh = (x - mean) * rstd;
+ * each may be NULL (not wanted). dx may be grad or x (same address and
+ * stride). The workspace is needed for dweight and dbias. */
+GIDS_API int gids_layer_norm_grad_workspace(int64_t n, int64_t dim, uint64_t *bytes);
+GIDS_API int gids_layer_norm_grad(int device, void *dx, int64_t dx_stride, void *dweight, void *dbias,
+                                  const void *grad, int64_t grad_stride, const void *x, int x_type, int64_t x_stride,
+                                  const void *weight, int param_type, const float *mean, const float *rstd, int64_t n,
+                                  int64_t dim, void *workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
