@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace gids {
 
@@ -95,6 +96,67 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
 #pragma unroll
   for (int i = 0; i < VEC; i++) r.v[i] = from_f32<T>(v[i]);
   store_raw(p, r);
+}
+
+// Asynchronous copy of 16 bytes to shared memory; zeros instead, and nothing
+// read, where `on` is false.
+__device__ __forceinline__ void copy_async(void* smem, const void* gmem, bool on) {
+  const unsigned int dst = (unsigned int)__cvta_generic_to_shared(smem);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(gmem), "r"(on ? 16 : 0) : "memory");
+}
+// The first `bytes` of 16, and zeros behind them.
+__device__ __forceinline__ void copy_async_tail(void* smem, const void* gmem, int bytes) {
+  const unsigned int dst = (unsigned int)__cvta_generic_to_shared(smem);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(gmem), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Two float32 values in one register pair: sm_100a adds, multiplies and fuses
+// both with one instruction, each half rounded as the scalar instruction does.
+struct F2 {
+  unsigned long long v;
+  F2() = default;
+  __device__ __forceinline__ F2(float lo, float hi) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  }
+  __device__ __forceinline__ explicit F2(float both) : F2(both, both) {}
+  __device__ __forceinline__ float lo() const { return __uint_as_float((unsigned int)v); }
+  __device__ __forceinline__ float hi() const { return __uint_as_float((unsigned int)(v >> 32)); }
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Elements 2 p and 2 p + 1 of K vectors laid end to end.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ F2 pair_of(const RowVec<T, VEC> (&v)[K], int p) {
+  if constexpr (VEC >= 2 && sizeof(T) == 2) {
+    const unsigned int u = reinterpret_cast<const unsigned int*>(&v[2 * p / VEC])[(2 * p % VEC) / 2];
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return F2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+      return F2(f.x, f.y);
+    }
+  } else {
+    return F2(to_f32(v[2 * p / VEC].v[2 * p % VEC]), to_f32(v[(2 * p + 1) / VEC].v[(2 * p + 1) % VEC]));
+  }
 }
 
 // n / d for 32-bit n by a multiplication (d >= 1 fixed at launch): with
