@@ -7,13 +7,11 @@
 //
 // Gradient: dweight[v, :] = round(scale * sum over {i : id_i = v} of grad[i, :]).
 // The ids are sorted (LSD radix sort of (id, position) words, stable, so equal
-// ids stay in position order), and the sorted list is cut into chunks of
-// CHUNK entries. A team of lanes owns one chunk and one slab of columns, walks
-// its entries with the running sum in registers, and stores a row of the
-// result whenever the id changes. A run of equal ids that crosses a chunk's
-// border leaves float32 partial sums in the workspace, which a second kernel
-// adds in chunk order. Nothing is accumulated with atomics, so results repeat
-// bit for bit. Padding and bad ids sort behind every row and are left out.
+// ids stay in position order) and the sorted list is cut into chunks whose runs
+// of equal ids are summed by a team of lanes each; sums of runs that cross
+// chunks are joined in a fixed order. Nothing is accumulated with atomics, so
+// results repeat bit for bit. Padding and bad ids sort behind every row and are
+// left out: their gradients are not read.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -91,6 +89,13 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_kernel(EmbArgs a) {
 }
 
 // ------------------------------------------------------------------ the sort
+// A chain of small kernels. Each is launched while the one before it drains
+// (programmatic launch) and waits for its results here.
+__device__ __forceinline__ void chain_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 constexpr int SORT_THREADS = 512;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_ITEMS = 4;
@@ -124,146 +129,189 @@ __device__ __forceinline__ unsigned long long source_word(const IdSource& s, uns
   return (key << 32) | i;
 }
 
-// counts[tile][digit] of one digit of the keys; tile t covers `per` words
-__global__ void __launch_bounds__(SORT_THREADS) count_kernel(IdSource src, unsigned int n, unsigned int per, int shift,
-                                                             int bits, unsigned int* __restrict__ counts) {
-  __shared__ unsigned int hist[MAX_RADIX];
-  const int radix = 1 << bits;
-  for (int d = threadIdx.x; d < radix; d += SORT_THREADS) hist[d] = 0;
+// Zeros for the rows of a dense gradient, written while the sort leaves the
+// memory idle: every kernel of the sort takes a share, as bulk copies of a zero
+// block of shared memory that run beside its own work. `bytes` and the
+// address are multiples of 16.
+constexpr int ZERO_BYTES = 8192;
+struct ZeroFill {
+  char* p;
+  unsigned long long bytes;
+};
+__device__ __forceinline__ void zero_begin(const ZeroFill& z, uint4* zeros) {
+  if (!z.bytes) return;
+  for (int i = threadIdx.x; i < ZERO_BYTES / 16; i += blockDim.x) zeros[i] = make_uint4(0, 0, 0, 0);
+  // the copies read shared memory through the asynchronous proxy
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
-  const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
-  for (unsigned int i = lo + threadIdx.x; i < hi; i += SORT_THREADS) {
-    const unsigned long long w = source_word(src, i);
-    atomicAdd(&hist[(unsigned int)(w >> shift) & (radix - 1)], 1u);
+  if (threadIdx.x != 0) return;
+  const unsigned int src = (unsigned int)__cvta_generic_to_shared(zeros);
+  for (unsigned long long at = (unsigned long long)blockIdx.x * ZERO_BYTES; at < z.bytes;
+       at += (unsigned long long)gridDim.x * ZERO_BYTES) {
+    const unsigned int b = (unsigned int)min((unsigned long long)ZERO_BYTES, z.bytes - at);
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(z.p + at), "r"(src), "r"(b)
+                 : "memory");
   }
-  __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += SORT_THREADS) counts[(size_t)blockIdx.x * radix + d] = hist[d];
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void zero_end(const ZeroFill& z) {
+  if (z.bytes && threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// Stable scatter of tile blockIdx.x by one digit: word order within a tile is
-// (step, warp, item, lane), which is the order of the positions.
-__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(IdSource src, unsigned int n, unsigned int per,
-                                                               unsigned int tiles, int shift, int bits,
-                                                               const unsigned int* __restrict__ counts,
-                                                               unsigned long long* __restrict__ out) {
-  __shared__ unsigned int base[MAX_RADIX];                   // next output index of each digit
-  __shared__ unsigned short wcount[SORT_WARPS][MAX_RADIX];   // digits of this step, by warp
-  __shared__ unsigned int wsum[SORT_WARPS];
-  const int radix = 1 << bits;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // base[d] = words of smaller digits + words of digit d in earlier tiles
-  unsigned int before = 0, total = 0;
-  if (tid < radix) {
-#pragma unroll 16
-    for (unsigned int t = 0; t < tiles; t++) {
-      const unsigned int c = counts[(size_t)t * radix + tid];
-      total += c;
-      before += t < blockIdx.x ? c : 0u;
+// counts[tile][digit] of one digit of the keys; tile t covers `per` words
+__global__ void __launch_bounds__(SORT_THREADS) count_kernel(IdSource src, unsigned int n, unsigned int per,
+                                                             unsigned int tiles, int shift, int bits,
+                                                             unsigned int* __restrict__ counts, ZeroFill zero) {
+  __shared__ unsigned int hist[MAX_RADIX];
+  __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
+  chain_wait();
+  zero_begin(zero, zeros);
+  if (blockIdx.x < tiles) {
+    const int radix = 1 << bits;
+    for (int d = threadIdx.x; d < radix; d += SORT_THREADS) hist[d] = 0;
+    __syncthreads();
+    const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
+    for (unsigned int i = lo + threadIdx.x; i < hi; i += SORT_THREADS) {
+      const unsigned long long w = source_word(src, i);
+      atomicAdd(&hist[(unsigned int)(w >> shift) & (radix - 1)], 1u);
     }
+    __syncthreads();
+    for (int d = threadIdx.x; d < radix; d += SORT_THREADS) counts[(size_t)blockIdx.x * radix + d] = hist[d];
   }
+  zero_end(zero);
+}
+
+struct SortShared {
+  unsigned int base[MAX_RADIX];                  // next output index of each digit
+  unsigned short wcount[SORT_WARPS][MAX_RADIX];  // digits of this step, by warp
+  unsigned int wsum[SORT_WARPS];
+};
+
+// base[d] = (words of smaller digits) + before, where thread d knows the words
+// `total` of digit d and `before`, those of them in earlier tiles
+__device__ __forceinline__ void digit_bases(SortShared& s, int radix, unsigned int total, unsigned int before) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned int incl = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) wsum[warp] = incl;
+  if (lane == 31) s.wsum[warp] = incl;
   __syncthreads();
   unsigned int off = 0;
-  for (int w = 0; w < warp; w++) off += wsum[w];
-  if (tid < radix) base[tid] = off + incl - total + before;
-
-  const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
-  for (unsigned int step = lo; step < hi; step += SORT_STEP) {
-    __syncthreads();
-    for (int i = tid; i < SORT_WARPS * MAX_RADIX / 2; i += SORT_THREADS)
-      reinterpret_cast<unsigned int*>(&wcount[0][0])[i] = 0;
-    __syncthreads();
-    unsigned long long word[SORT_ITEMS];
-    unsigned int rank[SORT_ITEMS];
-    unsigned int digit[SORT_ITEMS];
 #pragma unroll
-    for (int k = 0; k < SORT_ITEMS; k++) {
-      const unsigned int i = step + warp * (32 * SORT_ITEMS) + k * 32 + lane;
-      word[k] = i < hi ? source_word(src, i) : 0ull;
-      digit[k] = i < hi ? (unsigned int)(word[k] >> shift) & (radix - 1) : 0xffffffffu;
-    }
-#pragma unroll
-    for (int k = 0; k < SORT_ITEMS; k++) {
-      const unsigned int peers = __match_any_sync(0xffffffffu, digit[k]);
-      const bool in = digit[k] != 0xffffffffu;
-      const unsigned int prior = in ? wcount[warp][digit[k]] : 0u;
-      __syncwarp();
-      rank[k] = prior + __popc(peers & ((1u << lane) - 1u));
-      if (in && (peers >> lane) == 1u) wcount[warp][digit[k]] = (unsigned short)(prior + __popc(peers));
-      __syncwarp();
-    }
-    __syncthreads();
-    // by digit: warps' counts -> offsets within the step; base moves on
-    if (tid < radix) {
-      unsigned int run = 0;
-#pragma unroll
-      for (int w = 0; w < SORT_WARPS; w++) {
-        const unsigned int c = wcount[w][tid];
-        wcount[w][tid] = (unsigned short)run;
-        run += c;
-      }
-      total = run;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < SORT_ITEMS; k++)
-      if (digit[k] != 0xffffffffu) out[base[digit[k]] + wcount[warp][digit[k]] + rank[k]] = word[k];
-    __syncthreads();
-    if (tid < radix) base[tid] += total;
-  }
+  for (int w = 0; w < SORT_WARPS; w++) off += w < warp ? s.wsum[w] : 0u;
+  if (tid < radix) s.base[tid] = off + incl - total + before;
 }
 
-// --------------------------------------------------- the distinct ids, in order
-// A head is the first word of a run of equal keys (of rows: key < num_rows).
-__device__ __forceinline__ bool is_head(const unsigned long long* w, unsigned int i, unsigned int n,
-                                        unsigned long long num_rows) {
-  if (i >= n) return false;
+// Ranks SORT_ITEMS words a thread among the words of the same digit in this
+// step, in the order (warp, item, lane); leaves the step's count of digit d in
+// `total` of thread d and the warps' offsets in s.wcount.
+__device__ __forceinline__ void rank_step(SortShared& s, int radix, const unsigned int (&digit)[SORT_ITEMS],
+                                          unsigned int (&rank)[SORT_ITEMS], unsigned int& total) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = lane; i < (radix + 1) / 2; i += 32) reinterpret_cast<unsigned int*>(s.wcount[warp])[i] = 0;
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < SORT_ITEMS; k++) {
+    const unsigned int peers = __match_any_sync(0xffffffffu, digit[k]);
+    const bool in = digit[k] != 0xffffffffu;
+    const unsigned int prior = in ? s.wcount[warp][digit[k]] : 0u;
+    __syncwarp();
+    rank[k] = prior + __popc(peers & ((1u << lane) - 1u));
+    if (in && (peers >> lane) == 1u) s.wcount[warp][digit[k]] = (unsigned short)(prior + __popc(peers));
+    __syncwarp();
+  }
+  __syncthreads();
+  total = 0;
+  if (tid < radix) {
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; w++) {
+      const unsigned int c = s.wcount[w][tid];
+      s.wcount[w][tid] = (unsigned short)total;
+      total += c;
+    }
+  }
+  __syncthreads();
+}
+
+// Stable scatter of tile blockIdx.x by one digit.
+__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(IdSource src, unsigned int n, unsigned int per,
+                                                               unsigned int tiles, int shift, int bits,
+                                                               const unsigned int* __restrict__ counts,
+                                                               unsigned long long* __restrict__ out, ZeroFill zero) {
+  __shared__ SortShared s;
+  __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
+  chain_wait();
+  zero_begin(zero, zeros);
+  if (blockIdx.x < tiles) {
+    const int radix = 1 << bits;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned int before = 0, total = 0;
+    if (tid < radix) {
+      const unsigned int* c = counts + tid;
+#pragma unroll 37
+      for (unsigned int t = 0; t < tiles; t++) {
+        const unsigned int v = c[(size_t)t * radix];
+        total += v;
+        before += t < blockIdx.x ? v : 0u;
+      }
+    }
+    digit_bases(s, radix, total, before);
+    const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
+    for (unsigned int step = lo; step < hi; step += SORT_STEP) {
+      unsigned long long word[SORT_ITEMS];
+      unsigned int rank[SORT_ITEMS], digit[SORT_ITEMS];
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++) {
+        const unsigned int i = step + warp * (32 * SORT_ITEMS) + k * 32 + lane;
+        word[k] = i < hi ? source_word(src, i) : 0ull;
+        digit[k] = i < hi ? (unsigned int)(word[k] >> shift) & (radix - 1) : 0xffffffffu;
+      }
+      rank_step(s, radix, digit, rank, total);
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++)
+        if (digit[k] != 0xffffffffu) out[s.base[digit[k]] + s.wcount[warp][digit[k]] + rank[k]] = word[k];
+      __syncthreads();
+      if (tid < radix) s.base[tid] += total;
+    }
+  }
+  zero_end(zero);
+}
+
+// Runs: rank[i] = the runs of equal keys that start at or before word i, less
+// one, which is the result row of word i. Only words with a row (key <
+// num_rows) count.
+__device__ __forceinline__ bool is_head(const unsigned long long* w, unsigned int i, unsigned long long num_rows) {
   const unsigned long long k = w[i] >> 32;
   return k < num_rows && (i == 0 || (w[i - 1] >> 32) != k);
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) head_count_kernel(const unsigned long long* __restrict__ w,
-                                                                  unsigned int n, unsigned int per,
-                                                                  unsigned long long num_rows,
+__global__ void __launch_bounds__(SORT_THREADS) head_count_kernel(const unsigned long long* w, unsigned int n,
+                                                                  unsigned int per, unsigned long long num_rows,
                                                                   unsigned int* __restrict__ tile_heads) {
   __shared__ unsigned int sum;
+  chain_wait();
   if (threadIdx.x == 0) sum = 0;
   __syncthreads();
   const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
   unsigned int c = 0;
-  for (unsigned int i = lo + threadIdx.x; i < hi; i += SORT_THREADS) c += is_head(w, i, n, num_rows) ? 1u : 0u;
+  for (unsigned int i = lo + threadIdx.x; i < hi; i += SORT_THREADS) c += is_head(w, i, num_rows) ? 1u : 0u;
   for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
   if ((threadIdx.x & 31) == 0) atomicAdd(&sum, c);  // integers: the order does not matter
   __syncthreads();
   if (threadIdx.x == 0) tile_heads[blockIdx.x] = sum;
 }
 
-// chunk_rank[c] = heads before word c * chunk; *count = all heads
-__global__ void __launch_bounds__(SORT_THREADS) head_rank_kernel(const unsigned long long* __restrict__ w,
-                                                                 unsigned int n, unsigned int per, unsigned int tiles,
-                                                                 unsigned long long num_rows, unsigned int chunk_shift,
-                                                                 const unsigned int* __restrict__ tile_heads,
-                                                                 unsigned int* __restrict__ chunk_rank,
-                                                                 unsigned long long* __restrict__ count) {
-  __shared__ unsigned int wsum[SORT_WARPS];
+// Ranks of words [lo, hi) after `run` runs; returns the runs up to hi.
+__device__ __forceinline__ unsigned int rank_runs(const unsigned long long* w, unsigned int lo, unsigned int hi,
+                                                  unsigned long long num_rows, unsigned int run, unsigned int* wsum,
+                                                  unsigned int* rank) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned int run = 0, all = 0;
-  for (unsigned int t = 0; t < tiles; t++) {
-    const unsigned int c = tile_heads[t];
-    run += t < blockIdx.x ? c : 0u;
-    all += c;
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
-  const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
   for (unsigned int step = lo; step < hi; step += SORT_THREADS) {
     const unsigned int i = step + threadIdx.x;
-    const bool head = i < hi && is_head(w, i, n, num_rows);
+    const bool head = i < hi && is_head(w, i, num_rows);
     const unsigned int vote = __ballot_sync(0xffffffffu, head);
     __syncthreads();
     if (lane == 0) wsum[warp] = __popc(vote);
@@ -274,139 +322,307 @@ __global__ void __launch_bounds__(SORT_THREADS) head_rank_kernel(const unsigned 
       before += k < warp ? wsum[k] : 0u;
       sum += wsum[k];
     }
-    const unsigned int rank = before + __popc(vote & ((1u << lane) - 1u));
-    if (i < hi && (i & ((1u << chunk_shift) - 1u)) == 0) chunk_rank[i >> chunk_shift] = rank;
+    if (i < hi) rank[i] = before + __popc(vote & (0xffffffffu >> (31 - lane))) - 1u;
     run += sum;
   }
+  return run;
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) head_rank_kernel(const unsigned long long* w, unsigned int n,
+                                                                 unsigned int per, unsigned int tiles,
+                                                                 unsigned long long num_rows,
+                                                                 const unsigned int* tile_heads,
+                                                                 unsigned int* __restrict__ rank,
+                                                                 unsigned long long* __restrict__ count) {
+  __shared__ unsigned int wsum[SORT_WARPS];
+  __shared__ unsigned int heads[MAX_TILES];
+  chain_wait();
+  for (unsigned int t = threadIdx.x; t < tiles; t += SORT_THREADS) heads[t] = tile_heads[t];
+  __syncthreads();
+  unsigned int run = 0;
+  for (unsigned int t = 0; t < blockIdx.x; t++) run += heads[t];
+  const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
+  run = rank_runs(w, lo, hi, num_rows, run, wsum, rank);
+  if (blockIdx.x == tiles - 1 && threadIdx.x == 0) *count = run;
+}
+
+// A short list: block 0 sorts it in shared memory, pass by pass, and ranks its
+// runs (if `rank` is not null); the other blocks only write zeros.
+__global__ void __launch_bounds__(SORT_THREADS) small_sort_kernel(IdSource src, unsigned int n, int key_bits,
+                                                                  unsigned long long* __restrict__ out,
+                                                                  unsigned int* __restrict__ rank,
+                                                                  unsigned long long* __restrict__ count,
+                                                                  ZeroFill zero) {
+  __shared__ SortShared s;
+  __shared__ unsigned long long list[SORT_STEP];
+  __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
+  chain_wait();
+  zero_begin(zero, zeros);
+  if (blockIdx.x == 0) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned long long word[SORT_ITEMS];
+#pragma unroll
+    for (int k = 0; k < SORT_ITEMS; k++) {
+      const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
+      word[k] = i < n ? source_word(src, i) : ~0ull;
+    }
+    const int passes = (key_bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
+    int done = 0;
+    for (int p = 0; p < passes; p++) {
+      const int bits = (key_bits - done + (passes - p) - 1) / (passes - p), radix = 1 << bits;
+      unsigned int r[SORT_ITEMS], digit[SORT_ITEMS], total;
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++) {
+        const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
+        digit[k] = i < n ? (unsigned int)(word[k] >> (32 + done)) & (radix - 1) : 0xffffffffu;
+      }
+      rank_step(s, radix, digit, r, total);
+      digit_bases(s, radix, total, 0);
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++)
+        if (digit[k] != 0xffffffffu) list[s.base[digit[k]] + s.wcount[warp][digit[k]] + r[k]] = word[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++) {
+        const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
+        if (i < n) word[k] = list[i];
+      }
+      done += bits;
+      __syncthreads();
+    }
+    for (unsigned int i = tid; i < n; i += SORT_THREADS) out[i] = list[i];
+    if (rank) {
+      const unsigned int runs = rank_runs(list, 0, n, src.num_rows, 0, s.wsum, rank);
+      if (tid == 0) *count = runs;
+    }
+  }
+  zero_end(zero);
 }
 
 // ------------------------------------------------------------ sums over runs
+// A team of lanes walks a chunk of the sorted words for one slab of columns,
+// with the running sum in registers, and stores a row of the result where the
+// id changes. Sums of runs that cross the chunks of a block meet in shared
+// memory; those that cross blocks are left in the workspace for join_kernel.
+#ifndef SEG_U
+#define SEG_U 4
+#define SEG_BLOCKS 4
+#define SEG_MIN_CHUNK 4
+#endif
 constexpr int SEG_THREADS = 256;
-constexpr int SEG_UNROLL = 8;
 
 struct SegArgs {
   const unsigned long long* words;  // sorted
-  const unsigned int* chunk_rank;   // null: result rows are the keys (dense)
+  const unsigned int* rank;         // null: result rows are the keys (dense)
   void* out;
   const void* grad;
-  float* head;  // [chunks][dim] sums of runs that began in an earlier chunk
-  float* tail;  // [chunks][dim] sums of runs that go on in the next chunk
+  float* head;  // [blocks][dim] sums of runs that began in an earlier block
+  float* tail;  // [blocks][dim] sums of runs that go on in the next block
   long long out_stride, grad_stride;
-  unsigned long long num_rows, capacity;
+  unsigned int num_rows, capacity;
   long long dim;
-  long long* rows_out;  // with chunk_rank: the distinct keys, widened
-  unsigned int n, chunks, chunk_shift, team, slabs;
+  long long* rows_out;  // with rank: the distinct keys
+  unsigned int n, blocks, chunk, team, slabs;  // team: lanes, a power of two
   float scale;
 };
 
-template <typename W, int VEC>
-__device__ __forceinline__ void store_result(const SegArgs& a, unsigned long long row, long long col,
-                                             const float (&acc)[VEC]) {
-  float f[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; j++) f[j] = a.scale * acc[j];
-  store_vec<W, VEC>(reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride + col, f);
+__device__ __forceinline__ unsigned int key_of(const SegArgs& a, unsigned int i) {
+  return (unsigned int)(a.words[i] >> 32);
 }
 
-template <typename G, typename W, int VEC>
-__global__ void __launch_bounds__(SEG_THREADS) segment_kernel(SegArgs a) {
-  const unsigned long long item = ((unsigned long long)blockIdx.x * SEG_THREADS + threadIdx.x) / a.team;
-  const unsigned long long chunk64 = item / a.slabs;
-  if (chunk64 >= a.chunks) return;
-  const unsigned int chunk = (unsigned int)chunk64;
-  const unsigned int slab = (unsigned int)(item - chunk64 * a.slabs);
-  const long long col = ((long long)slab * a.team + (threadIdx.x & (a.team - 1))) * VEC;
-  if (col >= a.dim) return;
-  const unsigned int i0 = chunk << a.chunk_shift;
-  const unsigned int i1 = (unsigned int)min((unsigned long long)a.n, (unsigned long long)i0 + (1ull << a.chunk_shift));
-  unsigned long long cur = a.words[i0] >> 32;
-  if (cur >= a.num_rows) return;  // sorted: only padding and bad ids from here on
-  bool cont = i0 > 0 && (a.words[i0 - 1] >> 32) == cur;
-  // row of the run in hand; a run that began earlier is stored by the joiner
-  unsigned long long rank = a.chunk_rank ? a.chunk_rank[chunk] : 0ull;
-  if (cont) rank--;
-  float acc[VEC];
+// A thread has K vectors of VEC columns, vector k at column first + k * step.
+template <int VEC, int K>
+struct Columns {
+  long long first;
+  int step;
+  __device__ Columns(const SegArgs& a, unsigned int slab) {
+    first = ((long long)slab * a.team * K + (threadIdx.x & (a.team - 1))) * VEC;
+    step = (int)a.team * VEC;
+  }
+  __device__ __forceinline__ long long col(int k) const { return first + (long long)k * step; }
+};
+
+// the result row of the run that holds word `at`
+template <typename W, int VEC, int K>
+__device__ __forceinline__ void store_result(const SegArgs& a, const Columns<VEC, K>& c, unsigned int key,
+                                             unsigned int at, const float (&acc)[K][VEC]) {
+  const unsigned int row = a.rank ? a.rank[at] : key;
+  if (row >= a.capacity) return;
+  if (a.rank && c.first == 0) a.rows_out[row] = (long long)key;
+  W* out = reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride;
 #pragma unroll
-  for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
-  const G* g = reinterpret_cast<const G*>(a.grad);
-  const auto flush = [&] {
-    if (cont) {
-      store_vec<float, VEC>(a.head + (size_t)chunk * a.dim + col, acc);
-    } else {
-      const unsigned long long row = a.chunk_rank ? rank : cur;
-      if (row < a.capacity) {
-        store_result<W, VEC>(a, row, col, acc);
-        if (a.chunk_rank && col == 0) a.rows_out[row] = (long long)cur;
+  for (int k = 0; k < K; k++) {
+    if (c.col(k) >= a.dim) continue;
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) f[j] = a.scale * acc[k][j];
+    store_vec<W, VEC>(out + c.col(k), f);
+  }
+}
+
+template <int VEC, int K>
+__device__ __forceinline__ void store_partial(const SegArgs& a, const Columns<VEC, K>& c, float* row,
+                                              const float (&acc)[K][VEC]) {
+#pragma unroll
+  for (int k = 0; k < K; k++)
+    if (c.col(k) < a.dim) store_vec<float, VEC>(row + c.col(k), acc[k]);
+}
+
+template <int VEC, int K, typename F>
+__device__ __forceinline__ void each(F&& f) {
+#pragma unroll
+  for (int k = 0; k < K; k++)
+#pragma unroll
+    for (int j = 0; j < VEC; j++) f(k, j);
+}
+
+template <typename G, typename W, int VEC, int K>
+__global__ void __launch_bounds__(SEG_THREADS, SEG_BLOCKS) segment_kernel(SegArgs a) {
+  constexpr int U = SEG_U;  // words at a time; divides a chunk
+  constexpr unsigned int NONE = 0xffffffffu;
+  enum : unsigned char { CONT = 1, WHOLE = 2, TAIL = 4 };
+  __shared__ float heads[VEC * K][SEG_THREADS];  // sums of the runs that chunks start inside
+  // CONT: the chunk starts inside a run; WHOLE: and the run goes on behind it;
+  // TAIL: a run that starts in the chunk goes on behind it
+  __shared__ unsigned char flags[SEG_THREADS];
+  chain_wait();
+  const unsigned int block = blockIdx.x / a.slabs, slab = blockIdx.x - block * a.slabs;
+  const unsigned int teams = SEG_THREADS / a.team, me = threadIdx.x / a.team;
+  const Columns<VEC, K> c(a, slab);
+  const unsigned long long lo = ((unsigned long long)block * teams + me) * a.chunk;
+  const unsigned int i0 = (unsigned int)min(lo, (unsigned long long)a.n);
+  const unsigned int i1 = (unsigned int)min(lo + a.chunk, (unsigned long long)a.n);
+  float acc[K][VEC];
+  each<VEC, K>([&](int k, int j) { acc[k][j] = 0.0f; });
+  unsigned int cur = i0 < i1 ? key_of(a, i0) : NONE;
+  unsigned char flag = 0;
+  if (cur < a.num_rows) {
+    bool cont = i0 > 0 && key_of(a, i0 - 1) == cur;
+    if (cont) flag = CONT;
+    const G* g = reinterpret_cast<const G*>(a.grad) + c.first;
+    for (unsigned int i = i0; i < i1; i += U) {
+      unsigned int key[U], pos[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        // only the last chunk of all is not full: its last run ends there
+        const unsigned long long w = i + u < i1 ? a.words[i + u] : ~0ull;
+        key[u] = (unsigned int)(w >> 32);
+        pos[u] = (unsigned int)w;
+      }
+      RowVec<G, VEC> v[U][K];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+          if (key[u] < a.num_rows && c.col(k) < a.dim) {
+            v[u][k] = load_row<G, VEC>(g + (long long)pos[u] * a.grad_stride + k * c.step);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) v[u][k].v[j] = from_f32<G>(0.0f);
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (key[u] != cur && cur < a.num_rows) {  // the run in hand ends before word i + u
+          if (cont)
+            each<VEC, K>([&](int k, int j) { heads[k * VEC + j][threadIdx.x] = acc[k][j]; });
+          else
+            store_result<W, VEC, K>(a, c, cur, i + u - 1, acc);
+          cont = false;
+          cur = key[u];
+          each<VEC, K>([&](int k, int j) { acc[k][j] = 0.0f; });
+        }
+        each<VEC, K>([&](int k, int j) { acc[k][j] += to_f32(v[u][k].v[j]); });
       }
     }
+    if (cur < a.num_rows) {  // the run in hand at the chunk's end
+      const bool goes_on = i1 < a.n && key_of(a, i1) == cur;
+      if (cont) {
+        each<VEC, K>([&](int k, int j) { heads[k * VEC + j][threadIdx.x] = acc[k][j]; });
+        if (goes_on) flag |= WHOLE;
+      } else if (goes_on) {
+        flag |= TAIL;
+      } else {
+        store_result<W, VEC, K>(a, c, cur, i1 - 1, acc);
+      }
+    }
+  }
+  if ((threadIdx.x & (a.team - 1)) == 0) flags[me] = flag;
+  __syncthreads();
+  // adds the head sums of chunks k, k + 1, ... to acc up to the run's end;
+  // false if the run goes on behind the block
+  const auto follow = [&](unsigned int k) {
+    for (; k < teams; k++) {
+      const unsigned int t = k * a.team + (threadIdx.x & (a.team - 1));
+      each<VEC, K>([&](int q, int j) { acc[q][j] += heads[q * VEC + j][t]; });
+      if (!(flags[k] & WHOLE)) return true;
+    }
+    return false;
   };
-  for (unsigned int i = i0; i < i1; i += SEG_UNROLL) {
-    unsigned long long w[SEG_UNROLL];
-    RowVec<G, VEC> v[SEG_UNROLL];
-#pragma unroll
-    for (int u = 0; u < SEG_UNROLL; u++) w[u] = i + u < i1 ? a.words[i + u] : ~0ull;
-#pragma unroll
-    for (int u = 0; u < SEG_UNROLL; u++)
-      if ((w[u] >> 32) < a.num_rows)
-        v[u] = load_vec<G, VEC>(g + (long long)(unsigned int)w[u] * a.grad_stride + col);
-#pragma unroll
-    for (int u = 0; u < SEG_UNROLL; u++) {
-      const unsigned long long key = w[u] >> 32;
-      if (i + u < i1 && key != cur) {
-        flush();
-        cont = false;
-        cur = key;
-        rank++;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) acc[j] = 0.0f;
-        if (cur >= a.num_rows) return;
-      }
-      if (i + u < i1) {
-#pragma unroll
-        for (int j = 0; j < VEC; j++) acc[j] += to_f32(v[u].v[j]);
-      }
-    }
+  if (flag & TAIL) {
+    if (follow(me + 1))
+      store_result<W, VEC, K>(a, c, cur, i1 - 1, acc);
+    else
+      store_partial<VEC, K>(a, c, a.tail + (size_t)block * a.dim, acc);
   }
-  const bool goes_on = i1 < a.n && (a.words[i1] >> 32) == cur;
-  if (goes_on && !cont)
-    store_vec<float, VEC>(a.tail + (size_t)chunk * a.dim + col, acc);
-  else
-    flush();  // the run ends here, or fills the chunk between two others
+  if (me == 0 && (flag & CONT)) {
+    each<VEC, K>([&](int k, int j) { acc[k][j] = heads[k * VEC + j][threadIdx.x]; });
+    if (flag & WHOLE) follow(1);
+    store_partial<VEC, K>(a, c, a.head + (size_t)block * a.dim, acc);
+  }
 }
 
-// Runs that cross chunks: the team of the chunk where a run starts adds its
-// tail and the heads of the chunks it goes on in, in chunk order.
-template <typename W, int VEC>
+// Runs that cross blocks: the block where a run starts has its tail; the heads
+// of the blocks it goes on in are shared out over the teams and added in a
+// fixed order.
+template <typename W, int VEC, int K>
 __global__ void __launch_bounds__(SEG_THREADS) join_kernel(SegArgs a) {
-  const unsigned long long item = ((unsigned long long)blockIdx.x * SEG_THREADS + threadIdx.x) / a.team;
-  const unsigned long long chunk64 = item / a.slabs;
-  if (chunk64 + 1 >= a.chunks) return;  // the last chunk's runs end in it
-  const unsigned int chunk = (unsigned int)chunk64;
-  const unsigned int slab = (unsigned int)(item - chunk64 * a.slabs);
-  const long long col = ((long long)slab * a.team + (threadIdx.x & (a.team - 1))) * VEC;
-  if (col >= a.dim) return;
-  const unsigned int i0 = chunk << a.chunk_shift, i1 = (chunk + 1) << a.chunk_shift;
-  const unsigned long long cur = a.words[i1] >> 32;
-  if (cur >= a.num_rows || (a.words[i1 - 1] >> 32) != cur) return;
-  if ((a.words[i0] >> 32) == cur && i0 > 0 && (a.words[i0 - 1] >> 32) == cur) return;  // began earlier
-  float acc[VEC];
-  RowVec<float, VEC> v = load_vec<float, VEC>(a.tail + (size_t)chunk * a.dim + col);
+  __shared__ float sums[VEC * K][SEG_THREADS];
+  chain_wait();
+  const unsigned int block = blockIdx.x / a.slabs, slab = blockIdx.x - block * a.slabs;
+  if (block + 1 >= a.blocks) return;  // the last block's runs end in it
+  const unsigned int teams = SEG_THREADS / a.team, me = threadIdx.x / a.team;
+  const unsigned int rows = a.chunk * teams;
+  const unsigned int b0 = block * rows, b1 = b0 + rows;
+  const unsigned int cur = key_of(a, b1);
+  if (cur >= a.num_rows || key_of(a, b1 - 1) != cur) return;
+  if (b0 > 0 && key_of(a, b0) == cur && key_of(a, b0 - 1) == cur) return;  // it began earlier
+  // the blocks it goes on in: those that start with its key
+  unsigned int more = 0;
+  for (unsigned int base = block + 1;; base += SEG_THREADS) {
+    const unsigned int k = base + threadIdx.x;
+    const unsigned int some = __syncthreads_count(k < a.blocks && key_of(a, k * rows) == cur);
+    more += some;
+    if (some < SEG_THREADS) break;
+  }
+  const Columns<VEC, K> c(a, slab);
+  float acc[K][VEC];
+  each<VEC, K>([&](int k, int j) { acc[k][j] = 0.0f; });
+#pragma unroll 4
+  for (unsigned int h = me; h < more; h += teams) {
+    const float* row = a.head + (size_t)(block + 1 + h) * a.dim;
 #pragma unroll
-  for (int j = 0; j < VEC; j++) acc[j] = v.v[j];
-  for (unsigned int c = chunk + 1; c < a.chunks && (a.words[(size_t)c << a.chunk_shift] >> 32) == cur; c++) {
-    v = load_vec<float, VEC>(a.head + (size_t)c * a.dim + col);
+    for (int k = 0; k < K; k++) {
+      if (c.col(k) >= a.dim) continue;
+      const RowVec<float, VEC> v = load_row<float, VEC>(row + c.col(k));
 #pragma unroll
-    for (int j = 0; j < VEC; j++) acc[j] += v.v[j];
+      for (int j = 0; j < VEC; j++) acc[k][j] += v.v[j];
+    }
   }
-  unsigned long long row = cur;
-  if (a.chunk_rank) {  // heads up to and with this run's, less one
-    const unsigned int next = a.chunk_rank[chunk + 1];
-    row = (unsigned long long)next - 1ull;
+  each<VEC, K>([&](int k, int j) { sums[k * VEC + j][threadIdx.x] = acc[k][j]; });
+  __syncthreads();
+  if (me != 0) return;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    if (c.col(k) >= a.dim) continue;
+    const RowVec<float, VEC> v = load_row<float, VEC>(a.tail + (size_t)block * a.dim + c.col(k));
+#pragma unroll
+    for (int j = 0; j < VEC; j++) acc[k][j] = v.v[j];
   }
-  if (row < a.capacity) {
-    store_result<W, VEC>(a, row, col, acc);
-    if (a.chunk_rank && col == 0) a.rows_out[row] = (long long)cur;
-  }
+  for (unsigned int t = 0; t < teams && t < more; t++)
+    each<VEC, K>([&](int k, int j) { acc[k][j] += sums[k * VEC + j][t * a.team + threadIdx.x]; });
+  store_result<W, VEC, K>(a, c, cur, b1 - 1, acc);
 }
 
 // ------------------------------------------------------------------ host side
@@ -434,16 +650,35 @@ void check_device(int device) {
   GIDS_CHECK(device >= 0 && device < MAX_DEVICES, GIDS_E_INVAL, "bad device");
 }
 
-// Entries of a chunk: a border costs a partial row written and read, so longer
-// chunks for long lists; short ones where there are few words to share out.
-unsigned int chunk_shift_of(uint64_t n) { return n >= (1u << 18) ? 6 : 5; }
+// How the sums are cut: teams of lanes, K vectors of VEC elements a lane, and
+// chunks of words for a team.
+struct SegPlan {
+  unsigned int team, slabs, chunk, rows, blocks;  // rows: words of a block (all its teams)
+};
+SegPlan seg_plan(uint64_t n, uint64_t dim, int vec, int k) {
+  SegPlan p;
+  const uint64_t lanes = (dim + (uint64_t)vec * k - 1) / ((uint64_t)vec * k);
+  p.team = 1;
+  while (p.team < 32 && p.team < lanes) p.team <<= 1;
+  p.slabs = (unsigned int)((lanes + p.team - 1) / p.team);
+  const unsigned int teams = SEG_THREADS / p.team;
+  // long chunks leave fewer partial sums, short ones more work to share out:
+  // the longest that gives every SM three blocks
+  p.chunk = 32;
+  while (p.chunk > SEG_MIN_CHUNK && (n + p.chunk * teams - 1) / (p.chunk * teams) * p.slabs < 148 * 3) p.chunk >>= 1;
+  p.rows = p.chunk * teams;
+  p.blocks = (unsigned int)((n + p.rows - 1) / p.rows);
+  return p;
+}
+// vectors a lane for each vector length: 16 bytes of columns, or single elements
+constexpr int seg_k(int vec, int elem_bytes) { return vec * elem_bytes == 16 ? 1 : vec == 1 ? 16 / elem_bytes : 4 / elem_bytes; }
 
 struct Workspace {
-  uint64_t words_a, words_b, counts, tile_heads, count, chunk_rank, head, tail, bytes;
-  uint32_t chunks, chunk_shift;
+  uint64_t words_a, words_b, counts, tile_heads, count, rank, head, tail, bytes;
   Workspace(uint64_t n, uint64_t dim) {
-    chunk_shift = chunk_shift_of(n);
-    chunks = (uint32_t)((n + (1ull << chunk_shift) - 1) >> chunk_shift);
+    uint64_t blocks = 1;
+    for (const int e : {2, 4})
+      for (const int v : {1, 2, 16 / e}) blocks = std::max<uint64_t>(blocks, seg_plan(n, dim, v, seg_k(v, e)).blocks);
     uint64_t at = 0;
     const auto take = [&](uint64_t b) {
       const uint64_t here = at;
@@ -455,12 +690,27 @@ struct Workspace {
     words_b = take(n * 8);
     counts = take((uint64_t)MAX_TILES * MAX_RADIX * 4);
     tile_heads = take(MAX_TILES * 4);
-    chunk_rank = take(((uint64_t)chunks + 1) * 4);
-    head = take((uint64_t)chunks * dim * 4);
-    tail = take((uint64_t)chunks * dim * 4);
+    rank = take(n * 4);
+    head = take(blocks * dim * 4);
+    tail = take(blocks * dim * 4);
     bytes = at;
   }
 };
+
+// One kernel of a chain: all but the first start while the one before drains.
+template <typename... P, typename... A>
+void chain(bool first, void (*kernel)(P...), unsigned int grid, unsigned int block, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = first ? 0 : 1;
+  GIDS_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
 
 // tiles and words per tile of the sort of n words
 void sort_shape(uint64_t n, unsigned int* tiles, unsigned int* per) {
@@ -470,66 +720,94 @@ void sort_shape(uint64_t n, unsigned int* tiles, unsigned int* per) {
   *tiles = (unsigned int)((n + p - 1) / p);
 }
 
-int passes_of(uint64_t num_rows) {  // the largest key is num_rows
-  return std::max(1u, (bit_length(num_rows) + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS);
+int key_bits_of(uint64_t num_rows) { return std::max(1u, bit_length(num_rows)); }  // the largest key is num_rows
+int passes_of(uint64_t n, uint64_t num_rows) {
+  return n <= SORT_STEP ? 1 : (key_bits_of(num_rows) + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
+}
+uint64_t sorted_at(uint64_t n, uint64_t num_rows, const Workspace& lay) {
+  return (passes_of(n, num_rows) - 1) & 1 ? lay.words_b : lay.words_a;
 }
 
-// Sorts the ids into the workspace; returns where the sorted words are.
-unsigned long long* sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, cudaStream_t st) {
+// Sorts the ids into the workspace, writes `zero` meanwhile and, if asked,
+// ranks and counts the runs.
+void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks, int sms,
+              cudaStream_t st) {
+  unsigned int* rank = reinterpret_cast<unsigned int*>(ws + lay.rank);
+  unsigned long long* count = reinterpret_cast<unsigned long long*>(ws + lay.count);
+  const unsigned int fill_grid = zero.bytes ? (unsigned int)sms : 1;
+  if (n <= SORT_STEP) {
+    chain(true, small_sort_kernel, fill_grid, SORT_THREADS, st, ids, (unsigned int)n, key_bits_of(ids.num_rows),
+          reinterpret_cast<unsigned long long*>(ws + lay.words_a), ranks ? rank : nullptr, count, zero);
+    return;
+  }
   unsigned int tiles, per;
   sort_shape(n, &tiles, &per);
-  const int key_bits = std::max(1u, bit_length(ids.num_rows));
-  const int passes = passes_of(ids.num_rows);
+  const int key_bits = key_bits_of(ids.num_rows), passes = passes_of(n, ids.num_rows);
+  const unsigned int grid = std::max(tiles, fill_grid);
   unsigned long long* buf[2] = {reinterpret_cast<unsigned long long*>(ws + lay.words_a),
                                 reinterpret_cast<unsigned long long*>(ws + lay.words_b)};
   unsigned int* counts = reinterpret_cast<unsigned int*>(ws + lay.counts);
+  // an equal share of the zeros to every kernel
+  const uint64_t share = (zero.bytes / (2 * passes) + 15) / 16 * 16;
+  const auto next_share = [&] {
+    const ZeroFill z{zero.p, std::min<uint64_t>(share, zero.bytes)};
+    zero.p += z.bytes;
+    zero.bytes -= z.bytes;
+    return z;
+  };
   IdSource src = ids;
   int done = 0;
   for (int p = 0; p < passes; p++) {
     const int bits = (key_bits - done + (passes - p) - 1) / (passes - p);
-    count_kernel<<<tiles, SORT_THREADS, 0, st>>>(src, (unsigned int)n, per, 32 + done, bits, counts);
-    scatter_kernel<<<tiles, SORT_THREADS, 0, st>>>(src, (unsigned int)n, per, tiles, 32 + done, bits, counts,
-                                                   buf[p & 1]);
+    chain(p == 0, count_kernel, grid, SORT_THREADS, st, src, (unsigned int)n, per, tiles, 32 + done, bits, counts,
+          next_share());
+    chain(false, scatter_kernel, grid, SORT_THREADS, st, src, (unsigned int)n, per, tiles, 32 + done, bits,
+          (const unsigned int*)counts, buf[p & 1], next_share());
     src.id_bytes = 0;
     src.words = buf[p & 1];
     done += bits;
   }
-  return buf[(passes - 1) & 1];
+  if (!ranks) return;
+  unsigned int* heads = reinterpret_cast<unsigned int*>(ws + lay.tile_heads);
+  chain(false, head_count_kernel, tiles, SORT_THREADS, st, src.words, (unsigned int)n, per, ids.num_rows, heads);
+  chain(false, head_rank_kernel, tiles, SORT_THREADS, st, src.words, (unsigned int)n, per, tiles, ids.num_rows,
+        (const unsigned int*)heads, rank, count);
 }
 
 template <typename G, typename W, int VEC>
-void launch_segments(SegArgs a, cudaStream_t st) {
-  const uint64_t vecs = (uint64_t)a.dim / VEC;
-  a.team = 1;
-  while (a.team < 32 && a.team < vecs) a.team <<= 1;
-  a.slabs = (unsigned int)((vecs + a.team - 1) / a.team);
-  const uint64_t threads = (uint64_t)a.chunks * a.slabs * a.team;
-  const uint64_t blocks = (threads + SEG_THREADS - 1) / SEG_THREADS;
-  GIDS_CHECK(blocks < (1ull << 31), GIDS_E_UNSUPPORTED, "too many rows x columns for one launch");
-  segment_kernel<G, W, VEC><<<(unsigned int)blocks, SEG_THREADS, 0, st>>>(a);
-  if (a.chunks > 1) join_kernel<W, VEC><<<(unsigned int)blocks, SEG_THREADS, 0, st>>>(a);
-  GIDS_CUDA(cudaGetLastError());
+void launch_segments(SegArgs a, bool first, cudaStream_t st) {
+  constexpr int K = seg_k(VEC, sizeof(G));
+  const SegPlan p = seg_plan(a.n, (uint64_t)a.dim, VEC, K);
+  a.team = p.team;
+  a.slabs = p.slabs;
+  a.chunk = p.chunk;
+  a.blocks = p.blocks;
+  const uint64_t grid = (uint64_t)p.blocks * p.slabs;
+  GIDS_CHECK(grid < (1ull << 31), GIDS_E_UNSUPPORTED, "too many rows x columns for one launch");
+  chain(first, segment_kernel<G, W, VEC, K>, (unsigned int)grid, SEG_THREADS, st, a);
+  if (p.blocks > 1) chain(false, join_kernel<W, VEC, K>, (unsigned int)grid, SEG_THREADS, st, a);
 }
 
 template <typename G, typename W>
-void launch_segments_vec(const SegArgs& a, const Rows& out, const Rows& grad, cudaStream_t st) {
+void launch_segments_vec(const SegArgs& a, const Rows& out, const Rows& grad, bool first, cudaStream_t st) {
   constexpr int BIG = 16 / (int)sizeof(G);  // a 16-byte vector of the gradient
   if (vec_ok(out, a.dim, BIG) && vec_ok(grad, a.dim, BIG))
-    launch_segments<G, W, BIG>(a, st);
-  else if (vec_ok(out, a.dim, 2) && vec_ok(grad, a.dim, 2))
-    launch_segments<G, W, 2>(a, st);
+    launch_segments<G, W, BIG>(a, first, st);
+  else if (sizeof(G) == 2 && vec_ok(out, a.dim, 2) && vec_ok(grad, a.dim, 2))
+    launch_segments<G, W, sizeof(G) == 2 ? 2 : 1>(a, first, st);
   else
-    launch_segments<G, W, 1>(a, st);
+    launch_segments<G, W, 1>(a, first, st);
 }
 
-void segments(const SegArgs& a, const Rows& out, const Rows& grad, cudaStream_t st) {
+// first: nothing of this call was launched just before (the workspace is ready)
+void segments(const SegArgs& a, const Rows& out, const Rows& grad, bool first, cudaStream_t st) {
   if (out.type == GIDS_F32) {
-    if (grad.type == GIDS_F32) return launch_segments_vec<float, float>(a, out, grad, st);
-    if (grad.type == GIDS_F16) return launch_segments_vec<__half, float>(a, out, grad, st);
-    return launch_segments_vec<__nv_bfloat16, float>(a, out, grad, st);
+    if (grad.type == GIDS_F32) return launch_segments_vec<float, float>(a, out, grad, first, st);
+    if (grad.type == GIDS_F16) return launch_segments_vec<__half, float>(a, out, grad, first, st);
+    return launch_segments_vec<__nv_bfloat16, float>(a, out, grad, first, st);
   }
-  if (out.type == GIDS_F16) return launch_segments_vec<__half, __half>(a, out, grad, st);
-  return launch_segments_vec<__nv_bfloat16, __nv_bfloat16>(a, out, grad, st);
+  if (out.type == GIDS_F16) return launch_segments_vec<__half, __half>(a, out, grad, first, st);
+  return launch_segments_vec<__nv_bfloat16, __nv_bfloat16>(a, out, grad, first, st);
 }
 
 template <typename W, typename O, int VEC>
@@ -654,26 +932,32 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
   if (num_rows == 0 && n == 0) return;
   DeviceGuard dg(device);
   const size_t eb = (size_t)type_bytes(dweight.type);
-  if (num_rows > 0)
-    GIDS_CUDA(cudaMemset2DAsync(dweight.p, (num_rows > 1 ? (size_t)dweight.stride : (size_t)dim) * eb, 0,
-                                (size_t)dim * eb, (size_t)num_rows, st));
+  const uint64_t total = (uint64_t)num_rows * (uint64_t)dim * eb;
+  ZeroFill zero{static_cast<char*>(dweight.p), total};
+  // the zeros go out beside the sort if they are one aligned stretch of memory
+  if (n == 0 || (num_rows > 1 && dweight.stride != dim) || ((uintptr_t)dweight.p) % 16 || total % 16) {
+    zero.bytes = 0;
+    if (num_rows > 0)
+      GIDS_CUDA(cudaMemset2DAsync(dweight.p, (num_rows > 1 ? (size_t)dweight.stride : (size_t)dim) * eb, 0,
+                                  (size_t)dim * eb, (size_t)num_rows, st));
+  }
   if (n == 0) return;
   char* base = static_cast<char*>(ws);
+  sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, zero, false,
+           device_sms(device), st);
   SegArgs a{};
-  a.words = sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, st);
+  a.words = reinterpret_cast<const unsigned long long*>(base + sorted_at((uint64_t)n, (uint64_t)num_rows, lay));
   a.out = dweight.p;
   a.grad = grad.p;
   a.head = reinterpret_cast<float*>(base + lay.head);
   a.tail = reinterpret_cast<float*>(base + lay.tail);
   a.out_stride = dweight.stride;
   a.grad_stride = grad.stride;
-  a.num_rows = a.capacity = (unsigned long long)num_rows;
+  a.num_rows = a.capacity = (unsigned int)num_rows;
   a.dim = dim;
   a.n = (unsigned int)n;
-  a.chunks = lay.chunks;
-  a.chunk_shift = lay.chunk_shift;
   a.scale = scale;
-  segments(a, dweight, grad, st);
+  segments(a, dweight, grad, false, st);
 }
 
 void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
@@ -698,16 +982,8 @@ void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64
   if (n == 0) {
     GIDS_CUDA(cudaMemsetAsync(count, 0, sizeof(*count), st));
   } else {
-    const unsigned long long* w =
-        sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, st);
-    unsigned int tiles, per;
-    sort_shape((uint64_t)n, &tiles, &per);
-    unsigned int* th = reinterpret_cast<unsigned int*>(base + lay.tile_heads);
-    head_count_kernel<<<tiles, SORT_THREADS, 0, st>>>(w, (unsigned int)n, per, (unsigned long long)num_rows, th);
-    head_rank_kernel<<<tiles, SORT_THREADS, 0, st>>>(
-        w, (unsigned int)n, per, tiles, (unsigned long long)num_rows, lay.chunk_shift, th,
-        reinterpret_cast<unsigned int*>(base + lay.chunk_rank), count);
-    GIDS_CUDA(cudaGetLastError());
+    sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay,
+             ZeroFill{nullptr, 0}, true, 1, st);
   }
   if (count_dev) GIDS_CUDA(cudaMemcpyAsync(count_dev, count, sizeof(*count), cudaMemcpyDeviceToDevice, st));
   if (count_host) {
@@ -734,10 +1010,9 @@ void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacit
   if (n == 0 || capacity == 0) return;
   DeviceGuard dg(device);
   char* base = static_cast<char*>(ws);
-  const int passes = passes_of((uint64_t)num_rows);
   SegArgs a{};
-  a.words = reinterpret_cast<const unsigned long long*>(base + ((passes - 1) & 1 ? lay.words_b : lay.words_a));
-  a.chunk_rank = reinterpret_cast<const unsigned int*>(base + lay.chunk_rank);
+  a.words = reinterpret_cast<const unsigned long long*>(base + sorted_at((uint64_t)n, (uint64_t)num_rows, lay));
+  a.rank = reinterpret_cast<const unsigned int*>(base + lay.rank);
   a.rows_out = reinterpret_cast<long long*>(rows);
   a.out = values.p;
   a.grad = grad.p;
@@ -745,14 +1020,12 @@ void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacit
   a.tail = reinterpret_cast<float*>(base + lay.tail);
   a.out_stride = values.stride;
   a.grad_stride = grad.stride;
-  a.num_rows = (unsigned long long)num_rows;
-  a.capacity = (unsigned long long)capacity;
+  a.num_rows = (unsigned int)num_rows;
+  a.capacity = (unsigned int)std::min<int64_t>(capacity, n);
   a.dim = dim;
   a.n = (unsigned int)n;
-  a.chunks = lay.chunks;
-  a.chunk_shift = lay.chunk_shift;
   a.scale = scale;
-  segments(a, values, grad, st);
+  segments(a, values, grad, true, st);
 }
 
 void embedding_check(int device, cudaStream_t st) {
