@@ -26,7 +26,22 @@ import math
 
 import torch
 
-from .sampler import _store_module
+from .sampler import _store_module as _import_module
+
+try:  # the stream's handle without building a Stream object for every call
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:  # pragma: no cover - a build of torch without CUDA
+    _raw_stream = None
+
+_module = None
+
+
+def _store_module():
+    global _module
+    if _module is None:
+        _module = _import_module()
+    return _module
+
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -37,16 +52,16 @@ def _type(t: torch.dtype, what: str) -> int:
     return _TYPES[t]
 
 
-def _need_cuda(device: torch.device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _need_cuda(device: torch.device, *tensors):
     if device.type != "cuda":
         raise ValueError(f"CUDA tensors expected, not {device}")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"a tensor is on {t.device}, the others on {device}")
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
 
 
 def _check_ids(ids: torch.Tensor) -> torch.Tensor:
@@ -88,11 +103,11 @@ def _embedding_forward(ids, weight, scale, dtype):
         raise ValueError(f"weight must be a matrix, not {tuple(weight.shape)}")
     num_rows, dim = weight.shape
     wt, ot = _type(weight.dtype, "weight"), _type(dtype, "dtype")
-    _need_cuda(weight.device, ids=ids, weight=weight)
+    _need_cuda(weight.device, ids)
     if dim > 1 and weight.stride(1) != 1:
         raise ValueError("the columns of weight must be consecutive (stride 1)")
     ids = _check_ids(ids)
-    out = torch.empty((*ids.shape, dim), dtype=dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, dim), dtype=dtype)
     if dim:
         _store_module().embedding(weight.device.index, out.data_ptr(), ot, dim, weight.data_ptr(), wt,
                                   weight.stride(0), num_rows, dim, ids.data_ptr(), ids.element_size(), ids.numel(),
@@ -109,10 +124,9 @@ def _grad_args(ids, grad, num_rows, dtype):
         raise ValueError("grad has no columns")
     dtype = grad.dtype if dtype is None else dtype
     gt, wt = _type(grad.dtype, "grad"), _type(dtype, "dtype")
-    _need_cuda(grad.device, ids=ids, grad=grad)
+    _need_cuda(grad.device, ids)
     rows = _as_rows(grad, dim)
-    ws = torch.empty(_store_module().embedding_grad_workspace(ids.numel(), num_rows, dim), dtype=torch.uint8,
-                     device=grad.device)
+    ws = grad.new_empty(_store_module().embedding_grad_workspace(ids.numel(), num_rows, dim), dtype=torch.uint8)
     return ids, rows, dim, dtype, gt, wt, ws
 
 
@@ -124,7 +138,7 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None)
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
     ids, g, dim, dtype, gt, wt, ws = _grad_args(ids, grad, num_rows, dtype)
-    dw = torch.empty((num_rows, dim), dtype=dtype, device=grad.device)
+    dw = grad.new_empty((num_rows, dim), dtype=dtype)
     _store_module().embedding_grad(grad.device.index, dw.data_ptr(), wt, dim, num_rows, dim, g.data_ptr(), gt,
                                    g.stride(0), ids.data_ptr(), ids.element_size(), ids.numel(), pad, scale,
                                    ws.data_ptr(), ws.numel(), _stream(grad.device))
@@ -143,8 +157,8 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     n = ids.numel()
     count = m.embedding_group(dev.index, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
                               ws.numel(), 0, stream)
-    rows = torch.empty(count, dtype=torch.int64, device=dev)
-    values = torch.empty((count, dim), dtype=dtype, device=dev)
+    rows = grad.new_empty(count, dtype=torch.int64)
+    values = grad.new_empty((count, dim), dtype=dtype)
     m.embedding_grad_rows(dev.index, rows.data_ptr(), values.data_ptr(), wt, dim, count, num_rows, dim, g.data_ptr(),
                           gt, g.stride(0), n, scale, ws.data_ptr(), ws.numel(), stream)
     return rows, values
@@ -248,14 +262,14 @@ def _ptr(t) -> int:
 
 def _layer_norm_forward(x, weight, bias, eps, stats):
     dim, xt, pt = _params(x, weight, bias)
-    _need_cuda(x.device, x=x, weight=weight, bias=bias)
+    _need_cuda(x.device, weight, bias)
     rows = _as_rows(x, dim)
     n = rows.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     mean = rstd = None
     if stats:
-        mean = torch.empty(n, dtype=torch.float32, device=x.device)
-        rstd = torch.empty(n, dtype=torch.float32, device=x.device)
+        mean = x.new_empty(n, dtype=torch.float32)
+        rstd = x.new_empty(n, dtype=torch.float32)
     _store_module().layer_norm(x.device.index, y.data_ptr(), dim, _ptr(mean), _ptr(rstd), rows.data_ptr(), xt,
                                rows.stride(0), _ptr(weight), _ptr(bias), pt, n, dim, eps, _stream(x.device))
     return y, mean, rstd
@@ -275,7 +289,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
         pt = _TYPES[ptype]
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError(f"grad must be like x: {tuple(x.shape)} {x.dtype}, not {tuple(grad.shape)} {grad.dtype}")
-    _need_cuda(x.device, x=x, grad=grad, mean=mean, rstd=rstd, weight=weight)
+    _need_cuda(x.device, grad, mean, rstd, weight)
     xr, gr = _as_rows(x, dim), _as_rows(grad, dim)
     n = xr.shape[0]
     for name, s in (("mean", mean), ("rstd", rstd)):
@@ -283,10 +297,10 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
             raise ValueError(f"{name} must be a contiguous float32 tensor of {n} elements")
     m = _store_module()
     want_p = need[1] or need[2]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty(dim, dtype=ptype, device=x.device) if need[1] else None
-    db = torch.empty(dim, dtype=ptype, device=x.device) if need[2] else None
-    ws = torch.empty(m.layer_norm_grad_workspace(n, dim) if want_p else 0, dtype=torch.uint8, device=x.device)
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = x.new_empty(dim, dtype=ptype) if need[1] else None
+    db = x.new_empty(dim, dtype=ptype) if need[2] else None
+    ws = x.new_empty(m.layer_norm_grad_workspace(n, dim) if want_p else 0, dtype=torch.uint8)
     m.layer_norm_grad(x.device.index, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
                       gr.stride(0), xr.data_ptr(), xt, xr.stride(0), _ptr(weight), pt, mean.data_ptr(),
                       rstd.data_ptr(), n, dim, ws.data_ptr(), ws.numel(), _stream(x.device))

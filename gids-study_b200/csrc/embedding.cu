@@ -14,8 +14,10 @@
 // left out: their gradients are not read.
 #include <algorithm>
 #include <atomic>
+#include <map>
 #include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "layers.hpp"
 #include "rows.cuh"
@@ -96,10 +98,7 @@ __device__ __forceinline__ void chain_wait() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-constexpr int SORT_THREADS = 512;
-constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_ITEMS = 4;
-constexpr int SORT_STEP = SORT_THREADS * SORT_ITEMS;
 constexpr int MAX_DIGIT_BITS = 9;
 constexpr int MAX_RADIX = 1 << MAX_DIGIT_BITS;
 constexpr int MAX_TILES = 148;
@@ -158,38 +157,57 @@ __device__ __forceinline__ void zero_end(const ZeroFill& z) {
   if (z.bytes && threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// counts[tile][digit] of one digit of the keys; tile t covers `per` words
-__global__ void __launch_bounds__(SORT_THREADS) count_kernel(IdSource src, unsigned int n, unsigned int per,
-                                                             unsigned int tiles, int shift, int bits,
-                                                             unsigned int* __restrict__ counts, ZeroFill zero) {
+// A pass sorts by one digit of the keys: the bits [shift, shift + bits) of the
+// words. Tile t covers the words [t * per, (t + 1) * per).
+struct Pass {
+  unsigned int n, per, tiles;
+  int shift, bits;
+  unsigned int* counts;  // [tile][digit, at least 4] words
+};
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) count_kernel(IdSource src, Pass p, ZeroFill zero) {
   __shared__ unsigned int hist[MAX_RADIX];
   __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
   chain_wait();
   zero_begin(zero, zeros);
-  if (blockIdx.x < tiles) {
-    const int radix = 1 << bits;
-    for (int d = threadIdx.x; d < radix; d += SORT_THREADS) hist[d] = 0;
+  if (blockIdx.x < p.tiles) {
+    const int radix = 1 << p.bits;
+    const int row = max(radix, 4);
+    for (int d = threadIdx.x; d < row; d += THREADS) hist[d] = 0;
     __syncthreads();
-    const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
-    for (unsigned int i = lo + threadIdx.x; i < hi; i += SORT_THREADS) {
-      const unsigned long long w = source_word(src, i);
-      atomicAdd(&hist[(unsigned int)(w >> shift) & (radix - 1)], 1u);
+    const unsigned int lo = blockIdx.x * p.per, hi = min(p.n, lo + p.per);
+    for (unsigned int i0 = lo + threadIdx.x; i0 < hi; i0 += (THREADS * SORT_ITEMS)) {
+      unsigned int digit[SORT_ITEMS];
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++) {
+        const unsigned int i = i0 + k * THREADS;
+        digit[k] = i < hi ? (unsigned int)(source_word(src, i) >> p.shift) & (radix - 1) : (unsigned int)radix;
+      }
+#pragma unroll
+      for (int k = 0; k < SORT_ITEMS; k++)
+        if (digit[k] < (unsigned int)radix) atomicAdd(&hist[digit[k]], 1u);  // integers: the order does not matter
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < radix; d += SORT_THREADS) counts[(size_t)blockIdx.x * radix + d] = hist[d];
+    for (int d = threadIdx.x; d < row; d += THREADS) p.counts[blockIdx.x * row + d] = hist[d];
   }
   zero_end(zero);
 }
 
+template <int THREADS>
 struct SortShared {
   unsigned int base[MAX_RADIX];                  // next output index of each digit
-  unsigned short wcount[SORT_WARPS][MAX_RADIX];  // digits of this step, by warp
-  unsigned int wsum[SORT_WARPS];
+  unsigned int before[MAX_RADIX];                // words of the digit in earlier tiles
+  uint4 sum[2][THREADS];                    // shares of all words of 4 digits, and of those in earlier tiles
+  unsigned short wcount[(THREADS / 32)][MAX_RADIX];  // digits of this step, by warp
+  unsigned short part[4][MAX_RADIX];
+  unsigned int wsum[(THREADS / 32)];
 };
 
-// base[d] = (words of smaller digits) + before, where thread d knows the words
-// `total` of digit d and `before`, those of them in earlier tiles
-__device__ __forceinline__ void digit_bases(SortShared& s, int radix, unsigned int total, unsigned int before) {
+// base[d] = (words of smaller digits) + s.before[d], where thread d < radix
+// knows the number `total` of words of digit d
+template <int THREADS>
+__device__ __forceinline__ void digit_bases(SortShared<THREADS>& s, int radix, unsigned int total) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned int incl = total;
 #pragma unroll
@@ -200,81 +218,140 @@ __device__ __forceinline__ void digit_bases(SortShared& s, int radix, unsigned i
   if (lane == 31) s.wsum[warp] = incl;
   __syncthreads();
   unsigned int off = 0;
-#pragma unroll
-  for (int w = 0; w < SORT_WARPS; w++) off += w < warp ? s.wsum[w] : 0u;
-  if (tid < radix) s.base[tid] = off + incl - total + before;
+  for (int w = 0; w < warp && w < MAX_RADIX / 32; w++) off += s.wsum[w];
+  if (tid < radix) s.base[tid] = off + incl - total + s.before[tid];
 }
 
 // Ranks SORT_ITEMS words a thread among the words of the same digit in this
-// step, in the order (warp, item, lane); leaves the step's count of digit d in
-// `total` of thread d and the warps' offsets in s.wcount.
-__device__ __forceinline__ void rank_step(SortShared& s, int radix, const unsigned int (&digit)[SORT_ITEMS],
-                                          unsigned int (&rank)[SORT_ITEMS], unsigned int& total) {
+// step, in the order (warp, item, lane); returns the step's count of digit d to
+// thread d and leaves the warps' offsets in s.wcount.
+template <int THREADS>
+__device__ __forceinline__ unsigned int rank_step(SortShared<THREADS>& s, int radix, const unsigned int (&digit)[SORT_ITEMS],
+                                                  unsigned int (&rank)[SORT_ITEMS]) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = lane; i < (radix + 1) / 2; i += 32) reinterpret_cast<unsigned int*>(s.wcount[warp])[i] = 0;
   __syncwarp();
+  // lanes with the same digit: one ballot a bit
+  unsigned int peers[SORT_ITEMS];
+#pragma unroll
+  for (int k = 0; k < SORT_ITEMS; k++) peers[k] = __ballot_sync(0xffffffffu, digit[k] != 0xffffffffu);
+  for (int b = 0; (1 << b) < radix; b++) {
+#pragma unroll
+    for (int k = 0; k < SORT_ITEMS; k++) {
+      const bool one = (digit[k] >> b) & 1u;
+      const unsigned int vote = __ballot_sync(0xffffffffu, one);
+      peers[k] &= one ? vote : ~vote;
+    }
+  }
 #pragma unroll
   for (int k = 0; k < SORT_ITEMS; k++) {
-    const unsigned int peers = __match_any_sync(0xffffffffu, digit[k]);
     const bool in = digit[k] != 0xffffffffu;
     const unsigned int prior = in ? s.wcount[warp][digit[k]] : 0u;
     __syncwarp();
-    rank[k] = prior + __popc(peers & ((1u << lane) - 1u));
-    if (in && (peers >> lane) == 1u) s.wcount[warp][digit[k]] = (unsigned short)(prior + __popc(peers));
+    rank[k] = prior + __popc(peers[k] & ((1u << lane) - 1u));
+    if (in && (peers[k] >> lane) == 1u) s.wcount[warp][digit[k]] = (unsigned short)(prior + __popc(peers[k]));
     __syncwarp();
   }
   __syncthreads();
-  total = 0;
-  if (tid < radix) {
+  // the warps' counts become offsets: up to 4 threads to a digit, each with a
+  // share of the warps
+  const int parts = min(4, THREADS / radix), share = (THREADS / 32) / parts;
+  const int d = tid & (radix - 1), q = tid / radix;
+  constexpr int MOST = (THREADS / 32) * MAX_RADIX / THREADS;
+  unsigned short c[MOST];
+  unsigned int sum = 0;
+  if (q < parts) {
 #pragma unroll
-    for (int w = 0; w < SORT_WARPS; w++) {
-      const unsigned int c = s.wcount[w][tid];
-      s.wcount[w][tid] = (unsigned short)total;
-      total += c;
-    }
+    for (int w = 0; w < MOST; w++)
+      if (w < share) {
+        c[w] = s.wcount[q * share + w][d];
+        sum += c[w];
+      }
+    s.part[q][d] = (unsigned short)sum;
   }
   __syncthreads();
+  unsigned int total = 0;
+  if (q < parts) {
+    unsigned int run = 0;
+    for (int k = 0; k < parts; k++) {
+      const unsigned int v = s.part[k][d];
+      run += k < q ? v : 0u;
+      total += v;
+    }
+#pragma unroll
+    for (int w = 0; w < MOST; w++)
+      if (w < share) {
+        s.wcount[q * share + w][d] = (unsigned short)run;
+        run += c[w];
+      }
+  }
+  __syncthreads();
+  return total;
 }
 
 // Stable scatter of tile blockIdx.x by one digit.
-__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(IdSource src, unsigned int n, unsigned int per,
-                                                               unsigned int tiles, int shift, int bits,
-                                                               const unsigned int* __restrict__ counts,
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
                                                                unsigned long long* __restrict__ out, ZeroFill zero) {
-  __shared__ SortShared s;
+  extern __shared__ uint4 dyn[];
+  SortShared<THREADS>& s = *reinterpret_cast<SortShared<THREADS>*>(dyn);
   __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
   chain_wait();
   zero_begin(zero, zeros);
-  if (blockIdx.x < tiles) {
-    const int radix = 1 << bits;
+  if (blockIdx.x < p.tiles) {
+    const int radix = 1 << p.bits;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    unsigned int before = 0, total = 0;
-    if (tid < radix) {
-      const unsigned int* c = counts + tid;
-#pragma unroll 37
-      for (unsigned int t = 0; t < tiles; t++) {
-        const unsigned int v = c[(size_t)t * radix];
-        total += v;
-        before += t < blockIdx.x ? v : 0u;
-      }
-    }
-    digit_bases(s, radix, total, before);
-    const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
-    for (unsigned int step = lo; step < hi; step += SORT_STEP) {
-      unsigned long long word[SORT_ITEMS];
-      unsigned int rank[SORT_ITEMS], digit[SORT_ITEMS];
+    const unsigned int lo = blockIdx.x * p.per, hi = min(p.n, lo + p.per);
+    unsigned long long word[SORT_ITEMS];
+    unsigned int rank[SORT_ITEMS], digit[SORT_ITEMS];
+    const auto load = [&](unsigned int step) {
 #pragma unroll
       for (int k = 0; k < SORT_ITEMS; k++) {
         const unsigned int i = step + warp * (32 * SORT_ITEMS) + k * 32 + lane;
         word[k] = i < hi ? source_word(src, i) : 0ull;
-        digit[k] = i < hi ? (unsigned int)(word[k] >> shift) & (radix - 1) : 0xffffffffu;
+        digit[k] = i < hi ? (unsigned int)(word[k] >> p.shift) & (radix - 1) : 0xffffffffu;
       }
-      rank_step(s, radix, digit, rank, total);
+    };
+    load(lo);
+    // words of every digit in all tiles and in the earlier ones: a thread takes
+    // 4 digits and a share of the tiles (a digit's few instructions count here:
+    // one digit a thread took 3.5 us, this way 1.5)
+    const int quads = radix < 4 ? 1 : radix / 4, parts = THREADS / quads;
+    {
+      const int d = tid & (quads - 1), q = tid / quads;
+      uint4 all = make_uint4(0, 0, 0, 0), early = all;
+#pragma unroll 6
+      for (unsigned int t = q; t < p.tiles; t += parts) {
+        const uint4 v = reinterpret_cast<const uint4*>(p.counts)[t * quads + d];
+        all.x += v.x, all.y += v.y, all.z += v.z, all.w += v.w;
+        if (t < blockIdx.x) early.x += v.x, early.y += v.y, early.z += v.z, early.w += v.w;
+      }
+      s.sum[0][tid] = all;
+      s.sum[1][tid] = early;
+    }
+    __syncthreads();
+    unsigned int all = 0;
+    if (tid < radix) {
+      unsigned int early = 0;
+      const unsigned int* shares = reinterpret_cast<const unsigned int*>(s.sum);
+      for (int k = 0; k < parts && k < (int)p.tiles; k++) {
+        all += shares[k * quads * 4 + tid];
+        early += shares[(THREADS + k * quads) * 4 + tid];
+      }
+      s.before[tid] = early;
+    }
+    digit_bases(s, radix, all);
+    for (unsigned int step = lo; step < hi; step += (THREADS * SORT_ITEMS)) {
+      if (step != lo) load(step);
+      const unsigned int total = rank_step(s, radix, digit, rank);
 #pragma unroll
-      for (int k = 0; k < SORT_ITEMS; k++)
-        if (digit[k] != 0xffffffffu) out[s.base[digit[k]] + s.wcount[warp][digit[k]] + rank[k]] = word[k];
+      for (int k = 0; k < SORT_ITEMS; k++) {
+        if (digit[k] == 0xffffffffu) continue;
+        out[s.base[digit[k]] + s.wcount[warp][digit[k]] + rank[k]] = word[k];
+      }
       __syncthreads();
       if (tid < radix) s.base[tid] += total;
+      __syncthreads();
     }
   }
   zero_end(zero);
@@ -288,7 +365,8 @@ __device__ __forceinline__ bool is_head(const unsigned long long* w, unsigned in
   return k < num_rows && (i == 0 || (w[i - 1] >> 32) != k);
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) head_count_kernel(const unsigned long long* w, unsigned int n,
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) head_count_kernel(const unsigned long long* w, unsigned int n,
                                                                   unsigned int per, unsigned long long num_rows,
                                                                   unsigned int* __restrict__ tile_heads) {
   __shared__ unsigned int sum;
@@ -297,64 +375,80 @@ __global__ void __launch_bounds__(SORT_THREADS) head_count_kernel(const unsigned
   __syncthreads();
   const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
   unsigned int c = 0;
-  for (unsigned int i = lo + threadIdx.x; i < hi; i += SORT_THREADS) c += is_head(w, i, num_rows) ? 1u : 0u;
+#pragma unroll 4
+  for (unsigned int i = lo + threadIdx.x; i < hi; i += THREADS) c += is_head(w, i, num_rows) ? 1u : 0u;
   for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
   if ((threadIdx.x & 31) == 0) atomicAdd(&sum, c);  // integers: the order does not matter
   __syncthreads();
   if (threadIdx.x == 0) tile_heads[blockIdx.x] = sum;
 }
 
-// Ranks of words [lo, hi) after `run` runs; returns the runs up to hi.
+// Ranks of words [lo, hi) after `run` runs; returns the runs up to hi. Every
+// warp takes an equal stretch of words, counts its heads and then ranks them.
+template <int THREADS>
 __device__ __forceinline__ unsigned int rank_runs(const unsigned long long* w, unsigned int lo, unsigned int hi,
                                                   unsigned long long num_rows, unsigned int run, unsigned int* wsum,
                                                   unsigned int* rank) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (unsigned int step = lo; step < hi; step += SORT_THREADS) {
-    const unsigned int i = step + threadIdx.x;
-    const bool head = i < hi && is_head(w, i, num_rows);
-    const unsigned int vote = __ballot_sync(0xffffffffu, head);
-    __syncthreads();
-    if (lane == 0) wsum[warp] = __popc(vote);
-    __syncthreads();
-    unsigned int before = run, sum = 0;
+  const unsigned int stretch = ((hi - lo + (THREADS / 32) - 1) / (THREADS / 32) + 31) / 32 * 32;
+  const unsigned int a = min(hi, lo + warp * stretch), b = min(hi, a + stretch);
+  unsigned int mine = 0;
+#pragma unroll 4
+  for (unsigned int i = a; i < b; i += 32)
+    mine += __popc(__ballot_sync(0xffffffffu, i + lane < b && is_head(w, i + lane, num_rows)));
+  if (lane == 0) wsum[warp] = mine;
+  __syncthreads();
+  unsigned int before = run;
 #pragma unroll
-    for (int k = 0; k < SORT_WARPS; k++) {
-      before += k < warp ? wsum[k] : 0u;
-      sum += wsum[k];
-    }
-    if (i < hi) rank[i] = before + __popc(vote & (0xffffffffu >> (31 - lane))) - 1u;
-    run += sum;
+  for (int k = 0; k < (THREADS / 32); k++) {
+    before += k < warp ? wsum[k] : 0u;
+    run += wsum[k];
+  }
+#pragma unroll 4
+  for (unsigned int i = a; i < b; i += 32) {
+    const unsigned int vote = __ballot_sync(0xffffffffu, i + lane < b && is_head(w, i + lane, num_rows));
+    if (i + lane < b) rank[i + lane] = before + __popc(vote & (0xffffffffu >> (31 - lane))) - 1u;
+    before += __popc(vote);
   }
   return run;
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) head_rank_kernel(const unsigned long long* w, unsigned int n,
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) head_rank_kernel(const unsigned long long* w, unsigned int n,
                                                                  unsigned int per, unsigned int tiles,
                                                                  unsigned long long num_rows,
                                                                  const unsigned int* tile_heads,
                                                                  unsigned int* __restrict__ rank,
-                                                                 unsigned long long* __restrict__ count) {
-  __shared__ unsigned int wsum[SORT_WARPS];
-  __shared__ unsigned int heads[MAX_TILES];
+                                                                 unsigned long long* count,
+                                                                 volatile unsigned long long* host_count) {
+  __shared__ unsigned int wsum[(THREADS / 32)];
+  __shared__ unsigned int heads;
   chain_wait();
-  for (unsigned int t = threadIdx.x; t < tiles; t += SORT_THREADS) heads[t] = tile_heads[t];
+  if (threadIdx.x == 0) heads = 0;
   __syncthreads();
-  unsigned int run = 0;
-  for (unsigned int t = 0; t < blockIdx.x; t++) run += heads[t];
+  if (threadIdx.x < blockIdx.x) atomicAdd(&heads, tile_heads[threadIdx.x]);  // integers: the order does not matter
+  __syncthreads();
+  unsigned int run = heads;
   const unsigned int lo = blockIdx.x * per, hi = min(n, lo + per);
-  run = rank_runs(w, lo, hi, num_rows, run, wsum, rank);
-  if (blockIdx.x == tiles - 1 && threadIdx.x == 0) *count = run;
+  run = rank_runs<THREADS>(w, lo, hi, num_rows, run, wsum, rank);
+  if (blockIdx.x == tiles - 1 && threadIdx.x == 0) {
+    *count = run;
+    if (host_count) *host_count = run;
+  }
 }
 
 // A short list: block 0 sorts it in shared memory, pass by pass, and ranks its
 // runs (if `rank` is not null); the other blocks only write zeros.
-__global__ void __launch_bounds__(SORT_THREADS) small_sort_kernel(IdSource src, unsigned int n, int key_bits,
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) small_sort_kernel(IdSource src, unsigned int n, int key_bits,
                                                                   unsigned long long* __restrict__ out,
                                                                   unsigned int* __restrict__ rank,
-                                                                  unsigned long long* __restrict__ count,
+                                                                  unsigned long long* count,
+                                                                  volatile unsigned long long* host_count,
                                                                   ZeroFill zero) {
-  __shared__ SortShared s;
-  __shared__ unsigned long long list[SORT_STEP];
+  extern __shared__ uint4 dyn[];
+  SortShared<THREADS>& s = *reinterpret_cast<SortShared<THREADS>*>(dyn);
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn + (sizeof(SortShared<THREADS>) + 15) / 16);
   __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
   chain_wait();
   zero_begin(zero, zeros);
@@ -366,18 +460,19 @@ __global__ void __launch_bounds__(SORT_THREADS) small_sort_kernel(IdSource src, 
       const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
       word[k] = i < n ? source_word(src, i) : ~0ull;
     }
+    for (int d = tid; d < MAX_RADIX; d += THREADS) s.before[d] = 0;
     const int passes = (key_bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
     int done = 0;
     for (int p = 0; p < passes; p++) {
       const int bits = (key_bits - done + (passes - p) - 1) / (passes - p), radix = 1 << bits;
-      unsigned int r[SORT_ITEMS], digit[SORT_ITEMS], total;
+      unsigned int r[SORT_ITEMS], digit[SORT_ITEMS];
 #pragma unroll
       for (int k = 0; k < SORT_ITEMS; k++) {
         const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
         digit[k] = i < n ? (unsigned int)(word[k] >> (32 + done)) & (radix - 1) : 0xffffffffu;
       }
-      rank_step(s, radix, digit, r, total);
-      digit_bases(s, radix, total, 0);
+      const unsigned int total = rank_step(s, radix, digit, r);
+      digit_bases(s, radix, tid < radix ? total : 0u);
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < SORT_ITEMS; k++)
@@ -391,26 +486,31 @@ __global__ void __launch_bounds__(SORT_THREADS) small_sort_kernel(IdSource src, 
       done += bits;
       __syncthreads();
     }
-    for (unsigned int i = tid; i < n; i += SORT_THREADS) out[i] = list[i];
+    for (unsigned int i = tid; i < n; i += THREADS) out[i] = list[i];
     if (rank) {
-      const unsigned int runs = rank_runs(list, 0, n, src.num_rows, 0, s.wsum, rank);
-      if (tid == 0) *count = runs;
+      const unsigned int runs = rank_runs<THREADS>(list, 0, n, src.num_rows, 0, s.wsum, rank);
+      if (tid == 0) {
+        *count = runs;
+        if (host_count) *host_count = runs;
+      }
     }
   }
   zero_end(zero);
 }
 
 // ------------------------------------------------------------ sums over runs
-// A team of lanes walks a chunk of the sorted words for one slab of columns,
-// with the running sum in registers, and stores a row of the result where the
-// id changes. Sums of runs that cross the chunks of a block meet in shared
-// memory; those that cross blocks are left in the workspace for join_kernel.
-#ifndef SEG_U
-#define SEG_U 4
-#define SEG_BLOCKS 4
-#define SEG_MIN_CHUNK 4
-#endif
+// A team of lanes walks a chunk of the sorted words for one slab of columns (16
+// bytes of the gradient's row to a lane), with the running sum in registers,
+// and stores a row of the result where the id changes. Rows of the gradient
+// arrive through a ring of asynchronous copies, SEG_DEPTH - 1 rows ahead, which
+// keeps about 128 KB an SM in flight at few registers. Sums of runs that cross
+// the chunks of a block meet in shared memory; those that cross blocks are left
+// in the workspace for join_kernel.
 constexpr int SEG_THREADS = 256;
+constexpr unsigned int SEG_MAX_ROWS = 1024;  // words of a block
+#ifndef SEG_DEPTH
+#define SEG_DEPTH 8
+#endif
 
 struct SegArgs {
   const unsigned long long* words;  // sorted
@@ -431,7 +531,9 @@ __device__ __forceinline__ unsigned int key_of(const SegArgs& a, unsigned int i)
   return (unsigned int)(a.words[i] >> 32);
 }
 
-// A thread has K vectors of VEC columns, vector k at column first + k * step.
+// A thread has K vectors of VEC columns (16 bytes of the gradient), vector k at
+// column first + k * step: one vector where rows are aligned to it, else
+// single elements.
 template <int VEC, int K>
 struct Columns {
   long long first;
@@ -446,130 +548,165 @@ struct Columns {
 // the result row of the run that holds word `at`
 template <typename W, int VEC, int K>
 __device__ __forceinline__ void store_result(const SegArgs& a, const Columns<VEC, K>& c, unsigned int key,
-                                             unsigned int at, const float (&acc)[K][VEC]) {
+                                             unsigned int at, const F2 (&acc)[VEC * K / 2]) {
   const unsigned int row = a.rank ? a.rank[at] : key;
   if (row >= a.capacity) return;
   if (a.rank && c.first == 0) a.rows_out[row] = (long long)key;
   W* out = reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride;
+  const F2 scale(a.scale);
 #pragma unroll
   for (int k = 0; k < K; k++) {
     if (c.col(k) >= a.dim) continue;
     float f[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; j++) f[j] = a.scale * acc[k][j];
+    for (int j = 0; j < VEC; j++) {
+      const F2 v = mul2(scale, acc[(k * VEC + j) / 2]);
+      f[j] = (k * VEC + j) & 1 ? v.hi() : v.lo();
+    }
     store_vec<W, VEC>(out + c.col(k), f);
   }
 }
 
 template <int VEC, int K>
 __device__ __forceinline__ void store_partial(const SegArgs& a, const Columns<VEC, K>& c, float* row,
-                                              const float (&acc)[K][VEC]) {
+                                              const F2 (&acc)[VEC * K / 2]) {
 #pragma unroll
-  for (int k = 0; k < K; k++)
-    if (c.col(k) < a.dim) store_vec<float, VEC>(row + c.col(k), acc[k]);
-}
-
-template <int VEC, int K, typename F>
-__device__ __forceinline__ void each(F&& f) {
+  for (int k = 0; k < K; k++) {
+    if (c.col(k) >= a.dim) continue;
+    float f[VEC];
 #pragma unroll
-  for (int k = 0; k < K; k++)
-#pragma unroll
-    for (int j = 0; j < VEC; j++) f(k, j);
+    for (int j = 0; j < VEC; j++) f[j] = (k * VEC + j) & 1 ? acc[(k * VEC + j) / 2].hi() : acc[(k * VEC + j) / 2].lo();
+    store_vec<float, VEC>(row + c.col(k), f);
+  }
 }
 
 template <typename G, typename W, int VEC, int K>
-__global__ void __launch_bounds__(SEG_THREADS, SEG_BLOCKS) segment_kernel(SegArgs a) {
-  constexpr int U = SEG_U;  // words at a time; divides a chunk
+__global__ void __launch_bounds__(SEG_THREADS, 4) segment_kernel(SegArgs a) {
+  constexpr bool STAGED = VEC == 1;  // a team copies the 16-byte pieces that cover its columns
+  constexpr int P = VEC * K / 2, D = SEG_DEPTH;
   constexpr unsigned int NONE = 0xffffffffu;
   enum : unsigned char { CONT = 1, WHOLE = 2, TAIL = 4 };
-  __shared__ float heads[VEC * K][SEG_THREADS];  // sums of the runs that chunks start inside
+  extern __shared__ uint4 ring[];
+  __shared__ unsigned long long words[SEG_MAX_ROWS + 2];  // of the block, with the one before and the one behind
+  __shared__ F2 heads[P][SEG_THREADS];                    // sums of the runs that chunks start inside
   // CONT: the chunk starts inside a run; WHOLE: and the run goes on behind it;
   // TAIL: a run that starts in the chunk goes on behind it
   __shared__ unsigned char flags[SEG_THREADS];
-  chain_wait();
   const unsigned int block = blockIdx.x / a.slabs, slab = blockIdx.x - block * a.slabs;
-  const unsigned int teams = SEG_THREADS / a.team, me = threadIdx.x / a.team;
-  const Columns<VEC, K> c(a, slab);
-  const unsigned long long lo = ((unsigned long long)block * teams + me) * a.chunk;
-  const unsigned int i0 = (unsigned int)min(lo, (unsigned long long)a.n);
-  const unsigned int i1 = (unsigned int)min(lo + a.chunk, (unsigned long long)a.n);
-  float acc[K][VEC];
-  each<VEC, K>([&](int k, int j) { acc[k][j] = 0.0f; });
-  unsigned int cur = i0 < i1 ? key_of(a, i0) : NONE;
-  unsigned char flag = 0;
-  if (cur < a.num_rows) {
-    bool cont = i0 > 0 && key_of(a, i0 - 1) == cur;
-    if (cont) flag = CONT;
-    const G* g = reinterpret_cast<const G*>(a.grad) + c.first;
-    for (unsigned int i = i0; i < i1; i += U) {
-      unsigned int key[U], pos[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        // only the last chunk of all is not full: its last run ends there
-        const unsigned long long w = i + u < i1 ? a.words[i + u] : ~0ull;
-        key[u] = (unsigned int)(w >> 32);
-        pos[u] = (unsigned int)w;
-      }
-      RowVec<G, VEC> v[U][K];
-#pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-          if (key[u] < a.num_rows && c.col(k) < a.dim) {
-            v[u][k] = load_row<G, VEC>(g + (long long)pos[u] * a.grad_stride + k * c.step);
-          } else {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) v[u][k].v[j] = from_f32<G>(0.0f);
-          }
-        }
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        if (key[u] != cur && cur < a.num_rows) {  // the run in hand ends before word i + u
-          if (cont)
-            each<VEC, K>([&](int k, int j) { heads[k * VEC + j][threadIdx.x] = acc[k][j]; });
-          else
-            store_result<W, VEC, K>(a, c, cur, i + u - 1, acc);
-          cont = false;
-          cur = key[u];
-          each<VEC, K>([&](int k, int j) { acc[k][j] = 0.0f; });
-        }
-        each<VEC, K>([&](int k, int j) { acc[k][j] += to_f32(v[u][k].v[j]); });
-      }
-    }
-    if (cur < a.num_rows) {  // the run in hand at the chunk's end
-      const bool goes_on = i1 < a.n && key_of(a, i1) == cur;
-      if (cont) {
-        each<VEC, K>([&](int k, int j) { heads[k * VEC + j][threadIdx.x] = acc[k][j]; });
-        if (goes_on) flag |= WHOLE;
-      } else if (goes_on) {
-        flag |= TAIL;
-      } else {
-        store_result<W, VEC, K>(a, c, cur, i1 - 1, acc);
-      }
-    }
+  const unsigned int teams = SEG_THREADS / a.team, me = threadIdx.x / a.team, lane = threadIdx.x & (a.team - 1);
+  const unsigned int rows = a.chunk * teams;
+  const unsigned int b0 = block * rows;  // < n
+  const unsigned int here = min(rows, a.n - b0);
+  chain_wait();
+  // words[1 + i] is word b0 + i; a word without a row gets the key NONE
+  for (unsigned int i = threadIdx.x; i < rows + 2; i += SEG_THREADS) {
+    const bool in = i <= here + 1 && (i > 0 || b0 > 0) && (i <= here || b0 + here < a.n);
+    const unsigned long long w = in ? a.words[b0 + i - 1] : ~0ull;
+    words[i] = (unsigned int)(w >> 32) < a.num_rows ? w : ~0ull;
   }
-  if ((threadIdx.x & (a.team - 1)) == 0) flags[me] = flag;
+  __syncthreads();
+  const Columns<VEC, K> c(a, slab);
+  const unsigned long long* mine = words + 1 + me * a.chunk;
+  // ring slots: a thread's own vector, or its team's row of the slab
+  const int pitch = STAGED ? (SEG_THREADS + (int)teams) * 16 : SEG_THREADS * 16;
+  char* slot0 = reinterpret_cast<char*>(ring) + (STAGED ? me * (a.team + 1) * 16 : threadIdx.x * 16);
+  const char* g0 = reinterpret_cast<const char*>(a.grad) + (STAGED ? c.first - lane : c.first) * (long long)sizeof(G);
+  const long long row_bytes = a.grad_stride * (long long)sizeof(G);
+  const int slab_bytes = (int)min((long long)a.team * 16, (a.dim - (c.first - (STAGED ? lane : 0))) * (long long)sizeof(G));
+  const bool active = STAGED || c.first < a.dim;
+  const auto fetch = [&](unsigned int i) {
+    if (i < a.chunk) {
+      const unsigned long long w = mine[i];
+      if ((unsigned int)(w >> 32) != NONE && active) {
+        const char* src = g0 + (long long)(unsigned int)w * row_bytes;
+        char* dst = slot0 + (i & (D - 1)) * pitch;
+        if constexpr (STAGED) {
+          const int early = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+          for (int q = (int)lane * 16; q < early + slab_bytes; q += (int)a.team * 16)
+            copy_async_tail(dst + q, src - early + q, min(16, early + slab_bytes - q));
+        } else {
+          copy_async(dst, src, true);
+        }
+      }
+    }
+    copies_commit();
+  };
+  F2 acc[P];
+#pragma unroll
+  for (int p = 0; p < P; p++) acc[p] = F2(0.0f);
+#pragma unroll 1
+  for (unsigned int i = 0; i < D - 1; i++) fetch(i);
+  unsigned int cur = (unsigned int)(mine[0] >> 32);
+  bool cont = cur != NONE && (unsigned int)(mine[-1] >> 32) == cur;
+  unsigned char flag = cont ? CONT : 0;
+  // word i + 1 of the chunk decides what becomes of the sum after word i
+#pragma unroll 1
+  for (unsigned int i = 0; i < a.chunk; i++) {
+    if (STAGED) __syncwarp();  // the slot that fetch() refills has been read
+    fetch(i + D - 1);
+    copies_wait<D - 1>();
+    if (STAGED) __syncwarp();
+    if (cur == NONE) continue;
+    RowVec<G, VEC> v[K];
+    const char* src = slot0 + (i & (D - 1)) * pitch;
+    if constexpr (STAGED) {
+      const int early = (int)(((unsigned int)reinterpret_cast<uintptr_t>(g0) +
+                               (unsigned int)mine[i] * (unsigned int)row_bytes) & 15);
+#pragma unroll
+      for (int k = 0; k < K; k++)
+        v[k].v[0] = c.col(k) < a.dim
+                        ? *reinterpret_cast<const G*>(src + early + (k * a.team + lane) * (int)sizeof(G))
+                        : from_f32<G>(0.0f);
+    } else {
+      v[0] = *reinterpret_cast<const RowVec<G, VEC>*>(src);
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++) acc[p] = add2(acc[p], pair_of(v, p));
+    const unsigned int next = (unsigned int)(mine[i + 1] >> 32);
+    const bool last = i + 1 == a.chunk;
+    if (next == cur && !last) continue;
+    // the run ends here, or leaves the chunk
+    if (cont) {
+#pragma unroll
+      for (int p = 0; p < P; p++) heads[p][threadIdx.x] = acc[p];
+      if (next == cur) flag |= WHOLE;
+    } else if (next == cur) {
+      flag |= TAIL;
+      break;  // acc is the run's sum up to here
+    } else if (active) {
+      store_result<W, VEC, K>(a, c, cur, b0 + me * a.chunk + i, acc);
+    }
+    cont = false;
+    cur = next;
+#pragma unroll
+    for (int p = 0; p < P; p++) acc[p] = F2(0.0f);
+  }
+  copies_wait<0>();
+  if (lane == 0) flags[me] = flag;
   __syncthreads();
   // adds the head sums of chunks k, k + 1, ... to acc up to the run's end;
   // false if the run goes on behind the block
   const auto follow = [&](unsigned int k) {
     for (; k < teams; k++) {
-      const unsigned int t = k * a.team + (threadIdx.x & (a.team - 1));
-      each<VEC, K>([&](int q, int j) { acc[q][j] += heads[q * VEC + j][t]; });
+#pragma unroll
+      for (int p = 0; p < P; p++) acc[p] = add2(acc[p], heads[p][k * a.team + lane]);
       if (!(flags[k] & WHOLE)) return true;
     }
     return false;
   };
   if (flag & TAIL) {
-    if (follow(me + 1))
-      store_result<W, VEC, K>(a, c, cur, i1 - 1, acc);
-    else
+    const unsigned int at = b0 + (me + 1) * a.chunk - 1;  // the chunk's last word
+    if (follow(me + 1)) {
+      if (active) store_result<W, VEC, K>(a, c, (unsigned int)(words[1 + at - b0] >> 32), at, acc);
+    } else if (active) {
       store_partial<VEC, K>(a, c, a.tail + (size_t)block * a.dim, acc);
+    }
   }
   if (me == 0 && (flag & CONT)) {
-    each<VEC, K>([&](int k, int j) { acc[k][j] = heads[k * VEC + j][threadIdx.x]; });
+#pragma unroll
+    for (int p = 0; p < P; p++) acc[p] = heads[p][threadIdx.x];
     if (flag & WHOLE) follow(1);
-    store_partial<VEC, K>(a, c, a.head + (size_t)block * a.dim, acc);
+    if (active) store_partial<VEC, K>(a, c, a.head + (size_t)block * a.dim, acc);
   }
 }
 
@@ -578,9 +715,10 @@ __global__ void __launch_bounds__(SEG_THREADS, SEG_BLOCKS) segment_kernel(SegArg
 // fixed order.
 template <typename W, int VEC, int K>
 __global__ void __launch_bounds__(SEG_THREADS) join_kernel(SegArgs a) {
-  __shared__ float sums[VEC * K][SEG_THREADS];
-  chain_wait();
+  constexpr int P = VEC * K / 2;
+  __shared__ F2 sums[P][SEG_THREADS];
   const unsigned int block = blockIdx.x / a.slabs, slab = blockIdx.x - block * a.slabs;
+  chain_wait();
   if (block + 1 >= a.blocks) return;  // the last block's runs end in it
   const unsigned int teams = SEG_THREADS / a.team, me = threadIdx.x / a.team;
   const unsigned int rows = a.chunk * teams;
@@ -597,31 +735,35 @@ __global__ void __launch_bounds__(SEG_THREADS) join_kernel(SegArgs a) {
     if (some < SEG_THREADS) break;
   }
   const Columns<VEC, K> c(a, slab);
-  float acc[K][VEC];
-  each<VEC, K>([&](int k, int j) { acc[k][j] = 0.0f; });
-#pragma unroll 4
-  for (unsigned int h = me; h < more; h += teams) {
-    const float* row = a.head + (size_t)(block + 1 + h) * a.dim;
+  const auto add_row = [&](const float* row, F2 (&acc)[P]) {
+    RowVec<float, VEC> v[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      if (c.col(k) >= a.dim) continue;
-      const RowVec<float, VEC> v = load_row<float, VEC>(row + c.col(k));
+      if (c.col(k) < a.dim) {
+        v[k] = load_row<float, VEC>(row + c.col(k));
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) acc[k][j] += v.v[j];
+        for (int j = 0; j < VEC; j++) v[k].v[j] = 0.0f;
+      }
     }
-  }
-  each<VEC, K>([&](int k, int j) { sums[k * VEC + j][threadIdx.x] = acc[k][j]; });
+#pragma unroll
+    for (int p = 0; p < P; p++) acc[p] = add2(acc[p], pair_of(v, p));
+  };
+  F2 acc[P];
+#pragma unroll
+  for (int p = 0; p < P; p++) acc[p] = F2(0.0f);
+#pragma unroll 4
+  for (unsigned int h = me; h < more; h += teams) add_row(a.head + (size_t)(block + 1 + h) * a.dim, acc);
+#pragma unroll
+  for (int p = 0; p < P; p++) sums[p][threadIdx.x] = acc[p];
   __syncthreads();
-  if (me != 0) return;
+  if (me != 0 || c.first >= a.dim) return;
 #pragma unroll
-  for (int k = 0; k < K; k++) {
-    if (c.col(k) >= a.dim) continue;
-    const RowVec<float, VEC> v = load_row<float, VEC>(a.tail + (size_t)block * a.dim + c.col(k));
-#pragma unroll
-    for (int j = 0; j < VEC; j++) acc[k][j] = v.v[j];
-  }
+  for (int p = 0; p < P; p++) acc[p] = F2(0.0f);
+  add_row(a.tail + (size_t)block * a.dim, acc);
   for (unsigned int t = 0; t < teams && t < more; t++)
-    each<VEC, K>([&](int k, int j) { acc[k][j] += sums[k * VEC + j][t * a.team + threadIdx.x]; });
+#pragma unroll
+    for (int p = 0; p < P; p++) acc[p] = add2(acc[p], sums[p][t * a.team + threadIdx.x]);
   store_result<W, VEC, K>(a, c, cur, b1 - 1, acc);
 }
 
@@ -650,35 +792,30 @@ void check_device(int device) {
   GIDS_CHECK(device >= 0 && device < MAX_DEVICES, GIDS_E_INVAL, "bad device");
 }
 
-// How the sums are cut: teams of lanes, K vectors of VEC elements a lane, and
-// chunks of words for a team.
+// How the sums are cut: teams of lanes, and chunks of words for a team.
 struct SegPlan {
   unsigned int team, slabs, chunk, rows, blocks;  // rows: words of a block (all its teams)
 };
-SegPlan seg_plan(uint64_t n, uint64_t dim, int vec, int k) {
+SegPlan seg_plan(uint64_t n, uint64_t dim, int elem_bytes) {
   SegPlan p;
-  const uint64_t lanes = (dim + (uint64_t)vec * k - 1) / ((uint64_t)vec * k);
+  const uint64_t lanes = (dim * elem_bytes + 15) / 16;  // 16 bytes of a row to a lane
   p.team = 1;
   while (p.team < 32 && p.team < lanes) p.team <<= 1;
   p.slabs = (unsigned int)((lanes + p.team - 1) / p.team);
   const unsigned int teams = SEG_THREADS / p.team;
   // long chunks leave fewer partial sums, short ones more work to share out:
-  // the longest that gives every SM three blocks
-  p.chunk = 32;
-  while (p.chunk > SEG_MIN_CHUNK && (n + p.chunk * teams - 1) / (p.chunk * teams) * p.slabs < 148 * 3) p.chunk >>= 1;
+  // the longest that gives every SM four blocks
+  p.chunk = std::min(32u, SEG_MAX_ROWS / teams);
+  while (p.chunk > 4 && (n + p.chunk * teams - 1) / (p.chunk * teams) * p.slabs < 148 * 4) p.chunk >>= 1;
   p.rows = p.chunk * teams;
   p.blocks = (unsigned int)((n + p.rows - 1) / p.rows);
   return p;
 }
-// vectors a lane for each vector length: 16 bytes of columns, or single elements
-constexpr int seg_k(int vec, int elem_bytes) { return vec * elem_bytes == 16 ? 1 : vec == 1 ? 16 / elem_bytes : 4 / elem_bytes; }
 
 struct Workspace {
   uint64_t words_a, words_b, counts, tile_heads, count, rank, head, tail, bytes;
   Workspace(uint64_t n, uint64_t dim) {
-    uint64_t blocks = 1;
-    for (const int e : {2, 4})
-      for (const int v : {1, 2, 16 / e}) blocks = std::max<uint64_t>(blocks, seg_plan(n, dim, v, seg_k(v, e)).blocks);
+    const uint64_t blocks = std::max(seg_plan(n, dim, 2).blocks, seg_plan(n, dim, 4).blocks);
     uint64_t at = 0;
     const auto take = [&](uint64_t b) {
       const uint64_t here = at;
@@ -699,30 +836,40 @@ struct Workspace {
 
 // One kernel of a chain: all but the first start while the one before drains.
 template <typename... P, typename... A>
-void chain(bool first, void (*kernel)(P...), unsigned int grid, unsigned int block, cudaStream_t st, A... args) {
+void chain(bool first, void (*kernel)(P...), unsigned int grid, unsigned int block, size_t smem, cudaStream_t st,
+           A... args) {
+  if (smem > 24 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = first ? 0 : 1;
   GIDS_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
 }
 
+// Threads of the sort's blocks: more where every SM has more words than a step
+// of 512 threads takes (500,009 ids of 24 bits: 64 us with 1,024 threads, 73 with
+// 512; 16,384 tokens of 17 bits, dense: 76 and 66 us).
+constexpr uint64_t SMALL_LIST = 512 * SORT_ITEMS;
+bool wide_sort(uint64_t n) { return n > MAX_TILES * SMALL_LIST; }
+
 // tiles and words per tile of the sort of n words
 void sort_shape(uint64_t n, unsigned int* tiles, unsigned int* per) {
-  const uint64_t want = std::min<uint64_t>(MAX_TILES, (n + SORT_STEP - 1) / SORT_STEP);
-  const uint64_t p = ((n + want - 1) / want + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
+  const uint64_t threads = wide_sort(n) ? 1024 : 512, step = threads * SORT_ITEMS;
+  const uint64_t want = std::min<uint64_t>(MAX_TILES, (n + step - 1) / step);
+  const uint64_t p = ((n + want - 1) / want + threads - 1) / threads * threads;
   *per = (unsigned int)p;
   *tiles = (unsigned int)((n + p - 1) / p);
 }
 
 int key_bits_of(uint64_t num_rows) { return std::max(1u, bit_length(num_rows)); }  // the largest key is num_rows
 int passes_of(uint64_t n, uint64_t num_rows) {
-  return n <= SORT_STEP ? 1 : (key_bits_of(num_rows) + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
+  return n <= SMALL_LIST ? 1 : (key_bits_of(num_rows) + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
 }
 uint64_t sorted_at(uint64_t n, uint64_t num_rows, const Workspace& lay) {
   return (passes_of(n, num_rows) - 1) & 1 ? lay.words_b : lay.words_a;
@@ -730,14 +877,15 @@ uint64_t sorted_at(uint64_t n, uint64_t num_rows, const Workspace& lay) {
 
 // Sorts the ids into the workspace, writes `zero` meanwhile and, if asked,
 // ranks and counts the runs.
-void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks, int sms,
-              cudaStream_t st) {
+template <int THREADS>
+void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks,
+                 unsigned long long* count, unsigned long long* host_count, int sms, cudaStream_t st) {
   unsigned int* rank = reinterpret_cast<unsigned int*>(ws + lay.rank);
-  unsigned long long* count = reinterpret_cast<unsigned long long*>(ws + lay.count);
   const unsigned int fill_grid = zero.bytes ? (unsigned int)sms : 1;
-  if (n <= SORT_STEP) {
-    chain(true, small_sort_kernel, fill_grid, SORT_THREADS, st, ids, (unsigned int)n, key_bits_of(ids.num_rows),
-          reinterpret_cast<unsigned long long*>(ws + lay.words_a), ranks ? rank : nullptr, count, zero);
+  if (n <= SMALL_LIST) {
+    chain(true, small_sort_kernel<512>, fill_grid, 512, sizeof(SortShared<512>) + 16 + SMALL_LIST * 8, st, ids,
+          (unsigned int)n, key_bits_of(ids.num_rows), reinterpret_cast<unsigned long long*>(ws + lay.words_a),
+          ranks ? rank : nullptr, count, host_count, zero);
     return;
   }
   unsigned int tiles, per;
@@ -746,7 +894,6 @@ void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, Z
   const unsigned int grid = std::max(tiles, fill_grid);
   unsigned long long* buf[2] = {reinterpret_cast<unsigned long long*>(ws + lay.words_a),
                                 reinterpret_cast<unsigned long long*>(ws + lay.words_b)};
-  unsigned int* counts = reinterpret_cast<unsigned int*>(ws + lay.counts);
   // an equal share of the zeros to every kernel
   const uint64_t share = (zero.bytes / (2 * passes) + 15) / 16 * 16;
   const auto next_share = [&] {
@@ -756,36 +903,43 @@ void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, Z
     return z;
   };
   IdSource src = ids;
-  int done = 0;
+  Pass pass{(unsigned int)n, per, tiles, 32, 0, reinterpret_cast<unsigned int*>(ws + lay.counts)};
   for (int p = 0; p < passes; p++) {
-    const int bits = (key_bits - done + (passes - p) - 1) / (passes - p);
-    chain(p == 0, count_kernel, grid, SORT_THREADS, st, src, (unsigned int)n, per, tiles, 32 + done, bits, counts,
-          next_share());
-    chain(false, scatter_kernel, grid, SORT_THREADS, st, src, (unsigned int)n, per, tiles, 32 + done, bits,
-          (const unsigned int*)counts, buf[p & 1], next_share());
+    pass.shift += pass.bits;
+    pass.bits = (32 + key_bits - pass.shift + (passes - p) - 1) / (passes - p);
+    chain(p == 0, count_kernel<THREADS>, grid, THREADS, 0, st, src, pass, next_share());
+    chain(false, scatter_kernel<THREADS>, grid, THREADS, sizeof(SortShared<THREADS>), st, src, pass, buf[p & 1], next_share());
     src.id_bytes = 0;
     src.words = buf[p & 1];
-    done += bits;
   }
   if (!ranks) return;
   unsigned int* heads = reinterpret_cast<unsigned int*>(ws + lay.tile_heads);
-  chain(false, head_count_kernel, tiles, SORT_THREADS, st, src.words, (unsigned int)n, per, ids.num_rows, heads);
-  chain(false, head_rank_kernel, tiles, SORT_THREADS, st, src.words, (unsigned int)n, per, tiles, ids.num_rows,
-        (const unsigned int*)heads, rank, count);
+  chain(false, head_count_kernel<THREADS>, tiles, THREADS, 0, st, src.words, (unsigned int)n, per, ids.num_rows, heads);
+  chain(false, head_rank_kernel<THREADS>, tiles, THREADS, 0, st, src.words, (unsigned int)n, per, tiles, ids.num_rows,
+        (const unsigned int*)heads, rank, count, host_count);
+}
+
+void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks,
+              unsigned long long* count, unsigned long long* host_count, int sms, cudaStream_t st) {
+  if (wide_sort(n))
+    sort_ids_by<1024>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
+  else
+    sort_ids_by<512>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
 }
 
 template <typename G, typename W, int VEC>
 void launch_segments(SegArgs a, bool first, cudaStream_t st) {
-  constexpr int K = seg_k(VEC, sizeof(G));
-  const SegPlan p = seg_plan(a.n, (uint64_t)a.dim, VEC, K);
+  const SegPlan p = seg_plan(a.n, (uint64_t)a.dim, sizeof(G));
   a.team = p.team;
   a.slabs = p.slabs;
   a.chunk = p.chunk;
   a.blocks = p.blocks;
   const uint64_t grid = (uint64_t)p.blocks * p.slabs;
   GIDS_CHECK(grid < (1ull << 31), GIDS_E_UNSUPPORTED, "too many rows x columns for one launch");
-  chain(first, segment_kernel<G, W, VEC, K>, (unsigned int)grid, SEG_THREADS, st, a);
-  if (p.blocks > 1) chain(false, join_kernel<W, VEC, K>, (unsigned int)grid, SEG_THREADS, st, a);
+  constexpr int K = 16 / (VEC * (int)sizeof(G));
+  const size_t smem = (size_t)SEG_DEPTH * 16 * (SEG_THREADS + (VEC == 1 ? SEG_THREADS / p.team : 0));
+  chain(first, segment_kernel<G, W, VEC, K>, (unsigned int)grid, SEG_THREADS, smem, st, a);
+  if (p.blocks > 1) chain(false, join_kernel<W, VEC, K>, (unsigned int)grid, SEG_THREADS, 0, st, a);
 }
 
 template <typename G, typename W>
@@ -793,8 +947,6 @@ void launch_segments_vec(const SegArgs& a, const Rows& out, const Rows& grad, bo
   constexpr int BIG = 16 / (int)sizeof(G);  // a 16-byte vector of the gradient
   if (vec_ok(out, a.dim, BIG) && vec_ok(grad, a.dim, BIG))
     launch_segments<G, W, BIG>(a, first, st);
-  else if (sizeof(G) == 2 && vec_ok(out, a.dim, 2) && vec_ok(grad, a.dim, 2))
-    launch_segments<G, W, sizeof(G) == 2 ? 2 : 1>(a, first, st);
   else
     launch_segments<G, W, 1>(a, first, st);
 }
@@ -836,6 +988,31 @@ void launch_embedding_vec(const EmbArgs& a, const Rows& out, const Rows& weight,
     launch_embedding<W, O, 1>(a, n, dim, id_bytes, st);
 }
 
+// A word of mapped host memory for the time of a call that waits for its result.
+std::mutex g_words_mu;
+std::vector<unsigned long long*> g_words;
+struct HostWord {
+  unsigned long long *host = nullptr, *dev = nullptr;
+  explicit HostWord(bool wanted) {
+    if (!wanted) return;
+    {
+      std::lock_guard<std::mutex> lk(g_words_mu);
+      if (!g_words.empty()) {
+        host = g_words.back();
+        g_words.pop_back();
+      }
+    }
+    if (!host)
+      GIDS_CUDA(cudaHostAlloc(&host, sizeof(*host), cudaHostAllocMapped | cudaHostAllocPortable));
+    GIDS_CUDA(cudaHostGetDevicePointer(&dev, host, 0));
+  }
+  ~HostWord() {
+    if (!host) return;
+    std::lock_guard<std::mutex> lk(g_words_mu);
+    g_words.push_back(host);
+  }
+};
+
 IdSource id_source(const void* ids, int id_bytes, int64_t num_rows, int64_t padding_idx, int* err) {
   IdSource s{};
   s.ids = ids;
@@ -853,6 +1030,18 @@ void check_workspace(const void* ws, uint64_t ws_bytes, const Workspace& lay) {
 }
 
 }  // namespace
+
+void allow_smem(const void* kernel, size_t bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, size_t> allowed;
+  int dev = 0;
+  GIDS_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  size_t& most = allowed[{dev, kernel}];
+  if (bytes <= most) return;
+  GIDS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  most = bytes;
+}
 
 int* id_error_word(int device) {
   std::lock_guard<std::mutex> lk(g_err_mu);
@@ -944,7 +1133,7 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
   if (n == 0) return;
   char* base = static_cast<char*>(ws);
   sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, zero, false,
-           device_sms(device), st);
+           nullptr, nullptr, device_sms(device), st);
   SegArgs a{};
   a.words = reinterpret_cast<const unsigned long long*>(base + sorted_at((uint64_t)n, (uint64_t)num_rows, lay));
   a.out = dweight.p;
@@ -978,19 +1167,19 @@ void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64
                "count_host waits for the stream, which is being captured into a graph");
   }
   char* base = static_cast<char*>(ws);
-  unsigned long long* count = reinterpret_cast<unsigned long long*>(base + lay.count);
   if (n == 0) {
-    GIDS_CUDA(cudaMemsetAsync(count, 0, sizeof(*count), st));
-  } else {
-    sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay,
-             ZeroFill{nullptr, 0}, true, 1, st);
+    if (count_dev) GIDS_CUDA(cudaMemsetAsync(count_dev, 0, sizeof(*count_dev), st));
+    if (count_host) *count_host = 0;
+    return;
   }
-  if (count_dev) GIDS_CUDA(cudaMemcpyAsync(count_dev, count, sizeof(*count), cudaMemcpyDeviceToDevice, st));
+  HostWord word(count_host != nullptr);
+  unsigned long long* count =
+      count_dev ? reinterpret_cast<unsigned long long*>(count_dev) : reinterpret_cast<unsigned long long*>(base + lay.count);
+  sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay,
+           ZeroFill{nullptr, 0}, true, count, word.dev, 1, st);
   if (count_host) {
-    unsigned long long c = 0;
-    GIDS_CUDA(cudaMemcpyAsync(&c, count, sizeof(c), cudaMemcpyDeviceToHost, st));
     GIDS_CUDA(cudaStreamSynchronize(st));
-    *count_host = c;
+    *count_host = *reinterpret_cast<volatile unsigned long long*>(word.host);
   }
 }
 

@@ -689,11 +689,6 @@ constexpr int MAX_SMS = 256;  // the workspace is sized without a device
 // Partial rows of dw and db: one per block.
 int max_parts(int sms) { return std::min(sms, MAX_SMS); }
 
-void allow_smem(const void* kernel, size_t bytes) {
-  if (bytes > 40 * 1024)  // with the static part, more than a launch gets without asking
-    GIDS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-}
-
 // How the rows of a call's matrices meet 16-byte boundaries.
 struct Layout {
   bool alike = true;  // every matrix the same way
@@ -767,7 +762,7 @@ void launch_ln_k(LnArgs a, const Layout& l, int sms, cudaStream_t st) {
   // (plan_of has no full rows of single elements)
   const auto kernel = p.full ? ln_kernel<X, VEC, K, R, STAGES, (VEC > 1), LN_THREADS, GROUP>
                              : ln_kernel<X, VEC, K, R, STAGES, false, LN_THREADS, GROUP>;
-  allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (smem > 40 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<p.grid, dim3(p.group, p.groups), smem, st>>>(a);
 }
 
@@ -805,7 +800,7 @@ int launch_ln_grad_k(LnGradArgs a, const Layout& l, int sms, cudaStream_t st) {
                                p.groups > 1 ? (size_t)a.dim * 2 * sizeof(float) : 0);
   const auto kernel = p.full ? ln_grad_kernel<X, VEC, K, R, STAGES, (VEC > 1), LN_THREADS, GROUP>
                              : ln_grad_kernel<X, VEC, K, R, STAGES, false, LN_THREADS, GROUP>;
-  allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (smem > 40 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<p.grid, dim3(p.group, p.groups), smem, st>>>(a);
   return (int)p.grid;
 }

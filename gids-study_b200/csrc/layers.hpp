@@ -67,6 +67,10 @@ inline bool vec_ok(const Rows& r, int64_t dim, int vec) {
   return dim % vec == 0 && (r.stride * type_bytes(r.type)) % a == 0 && ((uintptr_t)r.p) % (uintptr_t)a == 0;
 }
 
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device.
+// What was allowed is remembered, for the runtime's call costs more than a launch.
+void allow_smem(const void* kernel, size_t bytes);
+
 inline int device_sms(int dev) {
   int sms = 0;
   GIDS_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
