@@ -1,9 +1,12 @@
 // Embedding lookup with scaling and its gradient by sorted ids, for sm_100a.
 //
-// Lookup: out[i, :] = round(scale * weight[id_i, :]). One thread moves UNROLL
-// vectors of a flat (row, vector) index space, so rows of any width fill the
-// warps; an id outside the table gives a zero row and sets the device's error
-// word.
+// Lookup: out[i, :] = round(scale * weight[id_i, :]). One thread moves
+// EMB_UNROLL vectors of a flat (row, vector) index space, so rows of any width
+// fill the warps; an id outside the table gives a zero row and sets the device's
+// error word. Rows that are not aligned to vectors come through shared memory
+// instead. Bound by HBM: 1,000,003 rows of 768 fp16 take 504 us, 0.94 of the
+// measured copy rate for the 3.07 GB they read and write (545 us when the output
+// stays in L2 and pushes out rows of the table).
 //
 // Gradient: dweight[v, :] = round(scale * sum over {i : id_i = v} of grad[i, :]).
 // The ids are sorted (LSD radix sort of (id, position) words, stable, so equal
@@ -78,16 +81,82 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_kernel(EmbArgs a) {
     O* o = reinterpret_cast<O*>(a.out) + (long long)row[u] * a.out_stride + (long long)col[u] * VEC;
     if constexpr (std::is_same<W, O>::value) {
       if (a.scale == 1.0f && good[u]) {  // a copy, NaN bits included
-        store_raw(o, v[u]);
+        store_stream(o, v[u]);
         continue;
       }
     }
-    float f[VEC];
+    RowVec<O, VEC> r;
 #pragma unroll
-    for (int j = 0; j < VEC; j++) f[j] = good[u] ? a.scale * to_f32(v[u].v[j]) : 0.0f;
+    for (int j = 0; j < VEC; j++) r.v[j] = from_f32<O>(good[u] ? a.scale * to_f32(v[u].v[j]) : 0.0f);
     if (!good[u]) *reinterpret_cast<volatile int*>(a.err) = 1;
-    store_vec<O, VEC>(o, f);
+    store_stream(o, r);
   }
+}
+
+// Rows that do not start on vectors: a warp fetches slabs of SLAB columns by the
+// aligned 16-byte pieces that cover them, ODD_STAGES - 1 slabs ahead, and
+// passes the elements on from shared memory. (200,000 rows of 1,001 bf16: 424 us
+// by single elements.)
+constexpr int ODD_SLAB = 512;
+constexpr int ODD_STAGES = 4;
+constexpr int ODD_THREADS = 256;
+
+template <typename W, typename O, typename ID>
+__global__ void __launch_bounds__(ODD_THREADS) embedding_odd_kernel(EmbArgs a, unsigned long long n, long long dim,
+                                                                    unsigned int slabs) {
+  constexpr int PITCH = ODD_SLAB * (int)sizeof(W) + 16;  // 16 bytes more, for a start inside a piece
+  extern __shared__ uint4 dyn[];
+  const unsigned int lane = threadIdx.x & 31;
+  char* ring = reinterpret_cast<char*>(dyn) + (threadIdx.x >> 5) * (PITCH * ODD_STAGES);
+  const unsigned long long total = n * slabs;
+  const unsigned long long step = (unsigned long long)gridDim.x * (ODD_THREADS / 32);
+  const unsigned long long first = (unsigned long long)blockIdx.x * (ODD_THREADS / 32) + (threadIdx.x >> 5);
+  const auto source = [&](unsigned long long unit, int& len) -> const char* {  // null: a bad id
+    const unsigned long long row = unit / slabs;
+    const long long c0 = (long long)(unit - row * slabs) * ODD_SLAB;
+    len = (int)min((long long)ODD_SLAB, dim - c0);
+    const unsigned long long id = load_id<ID>(a.ids, row);
+    if (id >= a.num_rows) return nullptr;
+    return reinterpret_cast<const char*>(reinterpret_cast<const W*>(a.weight) + (long long)id * a.weight_stride + c0);
+  };
+  const auto fetch = [&](unsigned long long unit, int stage) {
+    if (unit < total) {
+      int len;
+      const char* src = source(unit, len);
+      if (src) {
+        const int early = (int)(reinterpret_cast<uintptr_t>(src) & 15), span = early + len * (int)sizeof(W);
+        for (int q = (int)lane * 16; q < span; q += 512)
+          copy_async_tail(ring + stage * PITCH + q, src - early + q, min(16, span - q));
+      }
+    }
+    copies_commit();
+  };
+  for (int i = 0; i < ODD_STAGES - 1; i++) fetch(first + i * step, i);
+  int stage = 0;
+  for (unsigned long long unit = first; unit < total; unit += step) {
+    __syncwarp();  // the slot that fetch() refills has been read
+    fetch(unit + (ODD_STAGES - 1) * step, stage == 0 ? ODD_STAGES - 1 : stage - 1);
+    copies_wait<ODD_STAGES - 1>();
+    __syncwarp();
+    int len;
+    const char* src = source(unit, len);
+    const unsigned long long row = unit / slabs;
+    O* out = reinterpret_cast<O*>(a.out) + (long long)row * a.out_stride + (long long)(unit - row * slabs) * ODD_SLAB;
+    const W* in = reinterpret_cast<const W*>(ring + stage * PITCH + (reinterpret_cast<uintptr_t>(src) & 15));
+    if (!src && lane == 0) *reinterpret_cast<volatile int*>(a.err) = 1;
+#pragma unroll 4
+    for (int e = (int)lane; e < len; e += 32) {
+      if constexpr (std::is_same<W, O>::value) {
+        if (a.scale == 1.0f && src) {  // a copy, NaN bits included
+          out[e] = in[e];
+          continue;
+        }
+      }
+      out[e] = from_f32<O>(src ? a.scale * to_f32(in[e]) : 0.0f);
+    }
+    stage = stage + 1 == ODD_STAGES ? 0 : stage + 1;
+  }
+  copies_wait<0>();
 }
 
 // ------------------------------------------------------------------ the sort
@@ -980,12 +1049,20 @@ template <typename W, typename O>
 void launch_embedding_vec(const EmbArgs& a, const Rows& out, const Rows& weight, uint64_t n, int64_t dim, int id_bytes,
                           cudaStream_t st) {
   constexpr int BIG = 16 / (int)sizeof(W);  // a 16-byte vector of the table
-  if (vec_ok(out, dim, BIG) && vec_ok(weight, dim, BIG))
-    launch_embedding<W, O, BIG>(a, n, dim, id_bytes, st);
-  else if (vec_ok(out, dim, 2) && vec_ok(weight, dim, 2))
-    launch_embedding<W, O, 2>(a, n, dim, id_bytes, st);
-  else
-    launch_embedding<W, O, 1>(a, n, dim, id_bytes, st);
+  if (vec_ok(out, dim, BIG) && vec_ok(weight, dim, BIG)) return launch_embedding<W, O, BIG>(a, n, dim, id_bytes, st);
+  // a warp to a slab pays off from a few hundred bytes of row on
+  if (dim * (int64_t)sizeof(W) < 256) return launch_embedding<W, O, 1>(a, n, dim, id_bytes, st);
+  const uint64_t slabs = ((uint64_t)dim + ODD_SLAB - 1) / ODD_SLAB;
+  int dev = 0;
+  GIDS_CUDA(cudaGetDevice(&dev));
+  const size_t smem = (size_t)(ODD_SLAB * sizeof(W) + 16) * ODD_STAGES * (ODD_THREADS / 32);
+  const uint64_t want = (n * slabs + ODD_THREADS / 32 - 1) / (ODD_THREADS / 32);
+  const unsigned int grid =
+      (unsigned int)std::min<uint64_t>(want, (uint64_t)device_sms(dev) * (sizeof(W) == 4 ? 3 : 6));
+  const auto kernel = id_bytes == 4 ? embedding_odd_kernel<W, O, int> : embedding_odd_kernel<W, O, long long>;
+  if (smem > 40 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  kernel<<<grid, ODD_THREADS, smem, st>>>(a, n, dim, (unsigned int)slabs);
+  GIDS_CUDA(cudaGetLastError());
 }
 
 // A word of mapped host memory for the time of a call that waits for its result.

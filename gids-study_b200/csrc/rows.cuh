@@ -90,6 +90,16 @@ __device__ __forceinline__ void store_raw(T* p, const RowVec<T, VEC>& r) {
   for (int i = 0; i < N; i++) reinterpret_cast<P*>(p)[i] = reinterpret_cast<const P*>(&r)[i];
 }
 
+// The same for results that are not read again soon: they leave the L2 cache first.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_stream(T* p, const RowVec<T, VEC>& r) {
+  constexpr int B = sizeof(T) * VEC < 16 ? (int)sizeof(T) * VEC : 16;
+  using P = typename Piece<B>::type;
+  constexpr int N = (int)sizeof(T) * VEC / B;
+#pragma unroll
+  for (int i = 0; i < N; i++) __stcs(reinterpret_cast<P*>(p) + i, reinterpret_cast<const P*>(&r)[i]);
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   RowVec<T, VEC> r;
