@@ -109,13 +109,29 @@ class GIDS:
     nothing out), so that the gather, ``wb_size`` batches later, finds them
     resident; the reference's window buffering only protects marked pages
     from eviction.
+    The input layers of the model (``GIDS.layers``) can be given to the loader,
+    which applies them to every batch it hands out, on the current stream and
+    differentiable in their parameters. ``node_embeddings`` (heterographs; a
+    dict of node type -> ``layers.NodeEmbedding``) names the types that have no
+    stored features: their rows come from the learnable table instead of the
+    store. ``feature_norm`` (a ``layers.LayerNorm``, or in a heterograph a dict
+    of node type -> one) normalises the rows of the batch. Both run when the
+    batch is handed out, so with the accumulator they see the parameters of
+    that step, not those of the gather.
     """
 
     def __init__(self, page_size=4096, off=0, cache_dim=1024, num_ele=300 * 1000 * 1000 * 1024, num_ssd=1,
                  ssd_list=None, cache_size=10, ctrl_idx=0, window_buffer=False, wb_size=8, accumulator_flag=False,
                  long_type=False, heterograph=False, heterograph_map=None, *, dtype=None, ssd_capacity=0,
                  ssd_path=None, synchronous=False, shard_cache=False, process_group=None, cache_line=None,
-                 cache_admission=True, cache_ref_max=3, gather_blocks=0, wb_prefetch=False, replicas=0):
+                 cache_admission=True, cache_ref_max=3, gather_blocks=0, wb_prefetch=False, replicas=0,
+                 node_embeddings=None, feature_norm=None):
+        if node_embeddings and not heterograph:
+            raise ValueError("node_embeddings are for the node types of a heterograph (heterograph=True)")
+        if isinstance(feature_norm, dict) and not heterograph:
+            raise ValueError("feature_norm by node type needs a heterograph (heterograph=True)")
+        self.node_embeddings = dict(node_embeddings or {})
+        self.feature_norm = feature_norm
         if dtype is None:
             dtype = torch.int64 if long_type else torch.float32
         if dtype not in _STORE_CLASSES:
@@ -246,7 +262,7 @@ class GIDS:
         stream = _current_stream_handle(self.device)
         if self.heterograph:
             for key, value in batch[0].items():
-                if len(value) == 0:
+                if len(value) == 0 or key in self.node_embeddings:
                     continue
                 input_tensor = _as_index(value, self.device)
                 key_off = 0
@@ -297,7 +313,7 @@ class GIDS:
     def _batch_ids(self, batch):
         """(key offset, ids) of every node type of a batch."""
         if self.heterograph:
-            return [(self._key_off(k), v) for k, v in batch[0].items()]
+            return [(self._key_off(k), v) for k, v in batch[0].items() if k not in self.node_embeddings]
         return [(0, batch[0])]
 
     # ---------------------------------------------------------- replicated rows
@@ -374,6 +390,18 @@ class GIDS:
             print("Cannot find key: ", key, " in the heterograph map!")
         return 0
 
+    def _hand_out(self, batch, feat):
+        """The batch with its features, after the model's input layers (extension)."""
+        if self.node_embeddings:
+            for key, table in self.node_embeddings.items():
+                if key in feat:
+                    feat[key] = table(_as_index(batch[0][key], self.device))
+        if isinstance(self.feature_norm, dict):
+            feat = {k: self.feature_norm[k](v) if k in self.feature_norm else v for k, v in feat.items()}
+        elif self.feature_norm is not None:
+            feat = {k: self.feature_norm(v) for k, v in feat.items()} if self.heterograph else self.feature_norm(feat)
+        return _with_features(batch, feat)
+
     def fetch_feature(self, dim, it, device):
         """Next batch from ``it`` with its gathered features appended (GIDS.py:791-1058)."""
         GIDS_time_start = time.time()
@@ -396,6 +424,9 @@ class GIDS:
         if self.heterograph:
             ret_ten, outs, idxs, ns, keys = {}, [], [], [], []
             for key, v in batch[0].items():
+                if key in self.node_embeddings:
+                    ret_ten[key] = None  # looked up when the batch is handed out
+                    continue
                 if len(v) == 0:
                     ret_ten[key] = self._new_out(0, dim)
                     continue
@@ -408,13 +439,13 @@ class GIDS:
                 keys.append(self._key_off(key))
             self.BAM_FS.read_feature_hetero(len(outs), outs, idxs, ns, dim, self.cache_dim, keys, stream)
             self.GIDS_time += time.time() - GIDS_time_start
-            return _with_features(batch, ret_ten)
+            return self._hand_out(batch, ret_ten)
 
         index = _as_index(batch[0], self.device)
         out = self._new_out(len(index), dim)
         self.BAM_FS.read_feature(out.data_ptr(), index.data_ptr(), len(index), dim, self.cache_dim, 0, stream)
         self.GIDS_time += time.time() - GIDS_time_start
-        return _with_features(batch, out)
+        return self._hand_out(batch, out)
 
     def _fetch_accumulated(self, dim, it, stream, t0):
         """Storage Access Accumulator (GIDS.py:836-984): gather enough queued
@@ -423,11 +454,11 @@ class GIDS:
             return_ten = self.return_torch_buffer.pop(0)
             return_batch = self.window_buffer.pop(0)
             self.GIDS_time += time.time() - t0
-            return _with_features(return_batch, return_ten)
+            return self._hand_out(return_batch, return_ten)
 
         def n_access(b):
             if self.heterograph:
-                return sum(len(v) for v in b[0].values())
+                return sum(len(v) for k, v in b[0].items() if k not in self.node_embeddings)
             return len(b[0])
 
         buffer_size = len(self.window_buffer)
@@ -455,6 +486,9 @@ class GIDS:
             if self.heterograph:
                 ret_ten = {}
                 for k, v in batch[0].items():
+                    if k in self.node_embeddings:
+                        ret_ten[k] = None  # looked up when the batch is handed out
+                        continue
                     if len(v) == 0:
                         ret_ten[k] = self._new_out(0, dim)
                         continue
@@ -488,7 +522,7 @@ class GIDS:
         cpu_access_count = self.BAM_FS.get_cpu_access_count()
         self.prev_cpu_access = int(cpu_access_count / num_iter)
         self.BAM_FS.flush_cpu_access_count()
-        return _with_features(return_b, return_ten)
+        return self._hand_out(return_b, return_ten)
 
     # ---------------------------------------------------------------- stats
     def print_stats(self):

@@ -666,3 +666,50 @@ def test_other_device_than_the_current_one(layers):
         layers.layer_norm(w)
         layers.embedding_grad_rows(ids, w[ids], 50)
     assert torch.cuda.current_device() == 0
+
+
+def test_fetch_feature_trains_its_input_layers(layers):
+    """Gathered and embedded types through fetch_feature, a norm behind each, and
+    the gradients of a step, on the GPU."""
+    import numpy as np
+
+    import GIDS
+    from oracle import oracle
+
+    dim, rows = 96, 1000
+    t = oracle.synth_table(oracle.KIND_F32_UNIFORM, 3, rows, dim)
+    emb = layers.NodeEmbedding(500, dim, scale=2.0, sparse=True, device=DEV)
+    norms = {k: layers.LayerNorm(dim, device=DEV) for k in ("paper", "author")}
+    g = GIDS.GIDS(page_size=4096, cache_dim=dim, num_ele=t.size, num_ssd=2, cache_size=1, ctrl_idx=0, heterograph=True,
+                  heterograph_map={"paper": 0, "fos": 600}, node_embeddings={"author": emb}, feature_norm=norms,
+                  accumulator_flag=True)
+    g.required_accesses = 300
+    g.BAM_FS.write_range(t.ctypes.data, t.nbytes, 0)
+    rng = np.random.default_rng(0)
+    bs = [[{"paper": torch.as_tensor(rng.integers(0, 600, 150)), "author": torch.as_tensor(rng.integers(0, 500, 90)),
+            "fos": torch.as_tensor(rng.integers(0, 400, 60))}, f"s{i}"] for i in range(6)]
+    it = iter([list(b) for b in bs])
+    opt = torch.optim.SparseAdam([emb.weight], lr=0.1)
+    for b in bs[:3]:
+        table = emb.weight.detach().clone()
+        f = g.fetch_feature(dim, it, DEV)[-1]
+        paper = torch.as_tensor(oracle.gather(t, b[0]["paper"].numpy())).to(DEV)
+        fos = torch.as_tensor(oracle.gather(t, b[0]["fos"].numpy(), key_off=600)).to(DEV)
+        assert torch.equal(f["fos"], fos)
+        ref, _, _, err = norm_ref(paper, None, None, 1e-5)
+        close(f["paper"].detach(), ref, err)
+        ref, _, _, err = norm_ref(2.0 * table[b[0]["author"].to(DEV)], None, None, 1e-5)
+        close(f["author"].detach(), ref, err)
+        up = {k: randn(*f[k].shape, seed=5) for k in norms}
+        for k in norms:
+            norms[k].zero_grad(set_to_none=True)
+        opt.zero_grad(set_to_none=True)
+        torch.autograd.backward([f[k] for k in norms], [up[k] for k in norms])
+        for k in norms:
+            n = f[k].shape[0]
+            close(norms[k].bias.grad, up[k].double().sum(0), U * n * up[k].double().abs().sum(0))
+        grad = emb.weight.grad.coalesce()
+        assert torch.equal(grad.indices()[0], torch.unique(b[0]["author"]).to(DEV))
+        opt.step()
+        assert not torch.equal(emb.weight.detach(), table)  # the next batch sees the new rows
+    g.close()
