@@ -79,6 +79,11 @@ def _as_rows(t: torch.Tensor, dim: int) -> torch.Tensor:
     return t
 
 
+def _new_like(t: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _padding(padding_idx, num_rows: int) -> int:
     if padding_idx is None:
         return -1
@@ -265,7 +270,7 @@ def _layer_norm_forward(x, weight, bias, eps, stats):
     _need_cuda(x.device, weight, bias)
     rows = _as_rows(x, dim)
     n = rows.shape[0]
-    y = x.new_empty(x.shape)
+    y = _new_like(x)
     mean = rstd = None
     if stats:
         mean = x.new_empty(n, dtype=torch.float32)
@@ -297,7 +302,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
             raise ValueError(f"{name} must be a contiguous float32 tensor of {n} elements")
     m = _store_module()
     want_p = need[1] or need[2]
-    dx = x.new_empty(x.shape) if need[0] else None
+    dx = _new_like(x) if need[0] else None
     dw = x.new_empty(dim, dtype=ptype) if need[1] else None
     db = x.new_empty(dim, dtype=ptype) if need[2] else None
     ws = x.new_empty(m.layer_norm_grad_workspace(n, dim) if want_p else 0, dtype=torch.uint8)
