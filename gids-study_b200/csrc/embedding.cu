@@ -267,7 +267,6 @@ template <int THREADS>
 struct SortShared {
   unsigned int base[MAX_RADIX];                  // next output index of each digit
   unsigned int before[MAX_RADIX];                // words of the digit in earlier tiles
-  uint4 sum[2][THREADS];                    // shares of all words of 4 digits, and of those in earlier tiles
   unsigned short wcount[(THREADS / 32)][MAX_RADIX];  // digits of this step, by warp
   unsigned short part[4][MAX_RADIX];
   unsigned int wsum[(THREADS / 32)];
@@ -291,11 +290,12 @@ __device__ __forceinline__ void digit_bases(SortShared<THREADS>& s, int radix, u
   if (tid < radix) s.base[tid] = off + incl - total + s.before[tid];
 }
 
-// Ranks SORT_ITEMS words a thread among the words of the same digit in this
+// Ranks `items` words a thread among the words of the same digit in this
 // step, in the order (warp, item, lane); returns the step's count of digit d to
 // thread d and leaves the warps' offsets in s.wcount.
 template <int THREADS>
-__device__ __forceinline__ unsigned int rank_step(SortShared<THREADS>& s, int radix, const unsigned int (&digit)[SORT_ITEMS],
+__device__ __forceinline__ unsigned int rank_step(SortShared<THREADS>& s, int radix, int items,
+                                                  const unsigned int (&digit)[SORT_ITEMS],
                                                   unsigned int (&rank)[SORT_ITEMS]) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = lane; i < (radix + 1) / 2; i += 32) reinterpret_cast<unsigned int*>(s.wcount[warp])[i] = 0;
@@ -307,6 +307,7 @@ __device__ __forceinline__ unsigned int rank_step(SortShared<THREADS>& s, int ra
   for (int b = 0; (1 << b) < radix; b++) {
 #pragma unroll
     for (int k = 0; k < SORT_ITEMS; k++) {
+      if (k >= items) break;
       const bool one = (digit[k] >> b) & 1u;
       const unsigned int vote = __ballot_sync(0xffffffffu, one);
       peers[k] &= one ? vote : ~vote;
@@ -314,6 +315,7 @@ __device__ __forceinline__ unsigned int rank_step(SortShared<THREADS>& s, int ra
   }
 #pragma unroll
   for (int k = 0; k < SORT_ITEMS; k++) {
+    if (k >= items) break;
     const bool in = digit[k] != 0xffffffffu;
     const unsigned int prior = in ? s.wcount[warp][digit[k]] : 0u;
     __syncwarp();
@@ -364,6 +366,8 @@ __global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
                                                                unsigned long long* __restrict__ out, ZeroFill zero) {
   extern __shared__ uint4 dyn[];
   SortShared<THREADS>& s = *reinterpret_cast<SortShared<THREADS>*>(dyn);
+  // shares of all words of 4 digits, and of those in earlier tiles
+  uint4(*sum)[THREADS] = reinterpret_cast<uint4(*)[THREADS]>(dyn + (sizeof(SortShared<THREADS>) + 15) / 16);
   __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
   chain_wait();
   zero_begin(zero, zeros);
@@ -395,14 +399,14 @@ __global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
         all.x += v.x, all.y += v.y, all.z += v.z, all.w += v.w;
         if (t < blockIdx.x) early.x += v.x, early.y += v.y, early.z += v.z, early.w += v.w;
       }
-      s.sum[0][tid] = all;
-      s.sum[1][tid] = early;
+      sum[0][tid] = all;
+      sum[1][tid] = early;
     }
     __syncthreads();
     unsigned int all = 0;
     if (tid < radix) {
       unsigned int early = 0;
-      const unsigned int* shares = reinterpret_cast<const unsigned int*>(s.sum);
+      const unsigned int* shares = reinterpret_cast<const unsigned int*>(sum);
       for (int k = 0; k < parts && k < (int)p.tiles; k++) {
         all += shares[k * quads * 4 + tid];
         early += shares[(THREADS + k * quads) * 4 + tid];
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
     digit_bases(s, radix, all);
     for (unsigned int step = lo; step < hi; step += (THREADS * SORT_ITEMS)) {
       if (step != lo) load(step);
-      const unsigned int total = rank_step(s, radix, digit, rank);
+      const unsigned int total = rank_step(s, radix, SORT_ITEMS, digit, rank);
 #pragma unroll
       for (int k = 0; k < SORT_ITEMS; k++) {
         if (digit[k] == 0xffffffffu) continue;
@@ -506,65 +510,152 @@ __global__ void __launch_bounds__(THREADS) head_rank_kernel(const unsigned long 
   }
 }
 
-// A short list: block 0 sorts it in shared memory, pass by pass, and ranks its
-// runs (if `rank` is not null); the other blocks only write zeros.
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) small_sort_kernel(IdSource src, unsigned int n, int key_bits,
-                                                                  unsigned long long* __restrict__ out,
-                                                                  unsigned int* __restrict__ rank,
-                                                                  unsigned long long* count,
-                                                                  volatile unsigned long long* host_count,
-                                                                  ZeroFill zero) {
+// A short list: the blocks of a cluster sort it in their shared memory, with the
+// counts of a pass and then the words themselves exchanged between them, and
+// rank its runs (if `rank` is not null). Block c of the cluster has the words [c * tile, (c + 1) * tile), tile =
+// items * CLUSTER_THREADS.
+constexpr int CLUSTER_THREADS = 1024;
+constexpr int CLUSTER_BLOCKS = 8;
+struct ClusterShared {
+  SortShared<CLUSTER_THREADS> s;
+  unsigned int counts[MAX_RADIX];
+  unsigned int heads;
+  unsigned long long list[CLUSTER_THREADS * SORT_ITEMS];
+};
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of `p` (of this block's shared memory) in block `rank` of the cluster
+__device__ __forceinline__ unsigned int peer(const void* p, unsigned int rank) {
+  unsigned int r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r)
+               : "r"((unsigned int)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ unsigned int peer_load(const unsigned int* p, unsigned int rank) {
+  unsigned int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer(p, rank)) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(CLUSTER_THREADS) cluster_sort_kernel(IdSource src, unsigned int n, int key_bits,
+                                                                       int items, unsigned int blocks,
+                                                                       unsigned long long* __restrict__ out,
+                                                                       unsigned int* __restrict__ rank,
+                                                                       unsigned long long* count,
+                                                                       volatile unsigned long long* host_count) {
   extern __shared__ uint4 dyn[];
-  SortShared<THREADS>& s = *reinterpret_cast<SortShared<THREADS>*>(dyn);
-  unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn + (sizeof(SortShared<THREADS>) + 15) / 16);
-  __shared__ alignas(128) uint4 zeros[ZERO_BYTES / 16];
+  ClusterShared& c = *reinterpret_cast<ClusterShared*>(dyn);
+  SortShared<CLUSTER_THREADS>& s = c.s;
   chain_wait();
-  zero_begin(zero, zeros);
-  if (blockIdx.x == 0) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    unsigned long long word[SORT_ITEMS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const unsigned int me = blockIdx.x, tile = (unsigned int)items * CLUSTER_THREADS;
+  const unsigned int lo = me * tile;
+  const unsigned int mine = n > lo ? min(tile, n - lo) : 0;
+  const auto index = [&](int k) { return (unsigned int)(warp * 32 * items + k * 32 + lane); };
+  unsigned long long word[SORT_ITEMS];
+#pragma unroll
+  for (int k = 0; k < SORT_ITEMS; k++) word[k] = k < items && index(k) < mine ? source_word(src, lo + index(k)) : ~0ull;
+  const int passes = (key_bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
+  int done = 0;
+  for (int p = 0; p < passes; p++) {
+    const int bits = (key_bits - done + (passes - p) - 1) / (passes - p), radix = 1 << bits;
+    unsigned int r[SORT_ITEMS], digit[SORT_ITEMS];
+#pragma unroll
+    for (int k = 0; k < SORT_ITEMS; k++)
+      digit[k] = k < items && index(k) < mine ? (unsigned int)(word[k] >> (32 + done)) & (radix - 1) : 0xffffffffu;
+    const unsigned int total = rank_step(s, radix, items, digit, r);
+    if (tid < radix) c.counts[tid] = total;
+    cluster_sync();  // the counts are there; every list has been read
+    unsigned int all = 0;
+    if (tid < radix) {
+      unsigned int early = 0;
+#pragma unroll
+      for (unsigned int q = 0; q < CLUSTER_BLOCKS; q++) {
+        if (q >= blocks) break;
+        const unsigned int v = peer_load(&c.counts[tid], q);
+        all += v;
+        early += q < me ? v : 0u;
+      }
+      s.before[tid] = early;
+    }
+    digit_bases(s, radix, all);
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < SORT_ITEMS; k++) {
-      const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
-      word[k] = i < n ? source_word(src, i) : ~0ull;
+      if (digit[k] == 0xffffffffu) continue;
+      const unsigned int to = s.base[digit[k]] + s.wcount[warp][digit[k]] + r[k];  // < n
+      const unsigned int q = to / tile;
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer(&c.list[to - q * tile], q)), "l"(word[k]) : "memory");
     }
-    for (int d = tid; d < MAX_RADIX; d += THREADS) s.before[d] = 0;
-    const int passes = (key_bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
-    int done = 0;
-    for (int p = 0; p < passes; p++) {
-      const int bits = (key_bits - done + (passes - p) - 1) / (passes - p), radix = 1 << bits;
-      unsigned int r[SORT_ITEMS], digit[SORT_ITEMS];
+    cluster_sync();
 #pragma unroll
-      for (int k = 0; k < SORT_ITEMS; k++) {
-        const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
-        digit[k] = i < n ? (unsigned int)(word[k] >> (32 + done)) & (radix - 1) : 0xffffffffu;
+    for (int k = 0; k < SORT_ITEMS; k++)
+      if (k < items && index(k) < mine) word[k] = c.list[index(k)];
+    done += bits;
+  }
+#pragma unroll
+  for (int k = 0; k < SORT_ITEMS; k++)
+    if (k < items && index(k) < mine) out[lo + index(k)] = word[k];
+  if (rank) {
+    unsigned int votes[SORT_ITEMS], sum = 0;
+#pragma unroll
+    for (int k = 0; k < SORT_ITEMS; k++) {
+      bool head = false;
+      if (k < items && index(k) < mine) {
+        const unsigned int key = (unsigned int)(word[k] >> 32);
+        unsigned int before = 0xffffffffu;  // no key
+        if (index(k) > 0)
+          before = (unsigned int)(c.list[index(k) - 1] >> 32);
+        else if (me > 0)  // the high half of the last word of the block before
+          before = peer_load(reinterpret_cast<const unsigned int*>(&c.list[tile - 1]) + 1, me - 1);
+        head = key < src.num_rows && key != before;
       }
-      const unsigned int total = rank_step(s, radix, digit, r);
-      digit_bases(s, radix, tid < radix ? total : 0u);
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < SORT_ITEMS; k++)
-        if (digit[k] != 0xffffffffu) list[s.base[digit[k]] + s.wcount[warp][digit[k]] + r[k]] = word[k];
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < SORT_ITEMS; k++) {
-        const unsigned int i = warp * (32 * SORT_ITEMS) + k * 32 + lane;
-        if (i < n) word[k] = list[i];
-      }
-      done += bits;
-      __syncthreads();
+      votes[k] = __ballot_sync(0xffffffffu, head);
+      sum += __popc(votes[k]);
     }
-    for (unsigned int i = tid; i < n; i += THREADS) out[i] = list[i];
-    if (rank) {
-      const unsigned int runs = rank_runs<THREADS>(list, 0, n, src.num_rows, 0, s.wsum, rank);
-      if (tid == 0) {
-        *count = runs;
-        if (host_count) *host_count = runs;
-      }
+    if (lane == 0) s.wsum[warp] = sum;
+    __syncthreads();
+    unsigned int run = 0, heads = 0;
+#pragma unroll
+    for (int w = 0; w < CLUSTER_THREADS / 32; w++) {
+      run += w < warp ? s.wsum[w] : 0u;
+      heads += s.wsum[w];
+    }
+    if (tid == 0) c.heads = heads;
+    cluster_sync();
+    heads = 0;
+    for (unsigned int q = 0; q < blocks; q++) {
+      const unsigned int v = peer_load(&c.heads, q);
+      run += q < me ? v : 0u;
+      heads += v;
+    }
+#pragma unroll
+    for (int k = 0; k < SORT_ITEMS; k++) {
+      if (k < items && index(k) < mine)
+        rank[lo + index(k)] = run + __popc(votes[k] & (0xffffffffu >> (31 - lane))) - 1u;
+      run += __popc(votes[k]);
+    }
+    if (me == 0 && tid == 0) {
+      *count = heads;
+      if (host_count) *host_count = heads;
     }
   }
-  zero_end(zero);
+  cluster_sync();  // no block leaves while another may read its memory
+}
+
+// The zeros of a dense gradient beside cluster_sort_kernel, which leaves most
+// SMs free: this kernel starts with it and ends after it, so that the next one
+// in the chain finds both done.
+__global__ void __launch_bounds__(256) zero_kernel(ZeroFill z) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (unsigned long long at = ((unsigned long long)blockIdx.x * 256 + threadIdx.x) * 16; at < z.bytes;
+       at += (unsigned long long)gridDim.x * 256 * 16)
+    *reinterpret_cast<uint4*>(z.p + at) = zero;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ------------------------------------------------------------ sums over runs
@@ -1040,28 +1131,45 @@ struct Workspace {
 };
 
 // One kernel of a chain: all but the first start while the one before drains.
+struct Cluster {
+  unsigned int blocks;
+};
 template <typename... P, typename... A>
 void chain(bool first, void (*kernel)(P...), unsigned int grid, unsigned int block, size_t smem, cudaStream_t st,
-           A... args) {
+           Cluster cluster, A... args) {
   if (smem > 24 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2]{};
+  unsigned int attrs = 0;
+  if (!first) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster.blocks > 1) {
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = cluster.blocks;
+    attr[attrs].val.clusterDim.y = attr[attrs].val.clusterDim.z = 1;
+    attrs++;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = first ? 0 : 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = attrs;
   GIDS_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+template <typename... P, typename... A>
+void chain(bool first, void (*kernel)(P...), unsigned int grid, unsigned int block, size_t smem, cudaStream_t st,
+           A... args) {
+  chain(first, kernel, grid, block, smem, st, Cluster{1}, args...);
 }
 
 // Threads of the sort's blocks: more where every SM has more words than a step
 // of 512 threads takes (500,009 ids of 24 bits: 64 us with 1,024 threads, 73 with
 // 512; 16,384 tokens of 17 bits, dense: 76 and 66 us).
-constexpr uint64_t SMALL_LIST = 512 * SORT_ITEMS;
-bool wide_sort(uint64_t n) { return n > MAX_TILES * SMALL_LIST; }
+bool wide_sort(uint64_t n) { return n > (uint64_t)MAX_TILES * 512 * SORT_ITEMS; }
+constexpr uint64_t SMALL_LIST = (uint64_t)CLUSTER_BLOCKS * CLUSTER_THREADS * SORT_ITEMS;  // for one cluster
 
 // tiles and words per tile of the sort of n words
 void sort_shape(uint64_t n, unsigned int* tiles, unsigned int* per) {
@@ -1086,17 +1194,21 @@ template <int THREADS>
 void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks,
                  unsigned long long* count, unsigned long long* host_count, int sms, cudaStream_t st) {
   unsigned int* rank = reinterpret_cast<unsigned int*>(ws + lay.rank);
-  const unsigned int fill_grid = zero.bytes ? (unsigned int)sms : 1;
   if (n <= SMALL_LIST) {
-    chain(true, small_sort_kernel<512>, fill_grid, 512, sizeof(SortShared<512>) + 16 + SMALL_LIST * 8, st, ids,
-          (unsigned int)n, key_bits_of(ids.num_rows), reinterpret_cast<unsigned long long*>(ws + lay.words_a),
-          ranks ? rank : nullptr, count, host_count, zero);
+    // few words to a thread first, more blocks next, then more words
+    unsigned int items = 1, blocks = 1;
+    while (blocks < CLUSTER_BLOCKS && (uint64_t)blocks * CLUSTER_THREADS < n) blocks *= 2;
+    while ((uint64_t)blocks * CLUSTER_THREADS * items < n) items *= 2;
+    chain(true, cluster_sort_kernel, blocks, CLUSTER_THREADS, sizeof(ClusterShared), st, Cluster{blocks}, ids,
+          (unsigned int)n, key_bits_of(ids.num_rows), (int)items, blocks,
+          reinterpret_cast<unsigned long long*>(ws + lay.words_a), ranks ? rank : nullptr, count, host_count);
+    if (zero.bytes) chain(false, zero_kernel, (unsigned int)sms * 4, 256, 0, st, zero);
     return;
   }
   unsigned int tiles, per;
   sort_shape(n, &tiles, &per);
   const int key_bits = key_bits_of(ids.num_rows), passes = passes_of(n, ids.num_rows);
-  const unsigned int grid = std::max(tiles, fill_grid);
+  const unsigned int grid = std::max(tiles, zero.bytes ? (unsigned int)sms : 1u);
   unsigned long long* buf[2] = {reinterpret_cast<unsigned long long*>(ws + lay.words_a),
                                 reinterpret_cast<unsigned long long*>(ws + lay.words_b)};
   // an equal share of the zeros to every kernel
@@ -1113,7 +1225,8 @@ void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay
     pass.shift += pass.bits;
     pass.bits = (32 + key_bits - pass.shift + (passes - p) - 1) / (passes - p);
     chain(p == 0, count_kernel<THREADS>, grid, THREADS, 0, st, src, pass, next_share());
-    chain(false, scatter_kernel<THREADS>, grid, THREADS, sizeof(SortShared<THREADS>), st, src, pass, buf[p & 1], next_share());
+    chain(false, scatter_kernel<THREADS>, grid, THREADS,
+          sizeof(SortShared<THREADS>) + 16 + 2 * 16 * THREADS, st, src, pass, buf[p & 1], next_share());
     src.id_bytes = 0;
     src.words = buf[p & 1];
   }
