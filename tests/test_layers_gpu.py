@@ -713,3 +713,131 @@ def test_fetch_feature_trains_its_input_layers(layers):
         opt.step()
         assert not torch.equal(emb.weight.detach(), table)  # the next batch sees the new rows
     g.close()
+
+
+@pytest.mark.parametrize("n", [126, 127, 128, 129, 1024, 1025, 8191, 8192, 8193, 16384, 16385, 32767, 32768, 32769,
+                               303104, 303105])
+def test_grad_lengths_where_the_sort_changes(layers, n):
+    for seed, rows in enumerate((5, 3000, 1 << 18)):
+        check_grad(layers, randint(rows, (n,), seed=seed), randn(n, 8, seed=n, dtype="bf16"), rows, 1.0, 0,
+                   torch.float32)
+
+
+@pytest.mark.parametrize("dim", [1, 9, 129, 1024])
+def test_grad_few_hot_ids(layers, dim):
+    for n in (2, 33, 100, 128, 200):
+        for kind in range(3):
+            ids = torch.full((n,), 7, device=DEV)
+            if kind == 1:
+                ids[::3] = 2
+            if kind == 2:
+                ids[n // 2:] = torch.arange(n - n // 2, device=DEV) % 11
+            check_grad(layers, ids, randn(n, dim, seed=n, dtype="f16"), 11, 0.5, None)
+
+
+def test_odd_rows_and_bad_ids(layers):
+    for table, out in (("f32", "bf16"), ("f16", "f16")):
+        w = randn(300, 1030, dtype=table)[:, 1:1002]
+        for dt in (torch.int64, torch.int32):
+            ids = randint(300, (700,), dtype=dt)
+            check_embedding(layers, ids, w, 1.5, TYPES[out])
+            ids[5], ids[699] = 300, -1
+            got = layers.embedding(ids, w, scale=1.5, dtype=TYPES[out])
+            with pytest.raises(RuntimeError, match="outside its table"):
+                layers.check_ids(DEV)
+            assert not got[5].any() and not got[699].any()
+            close(got[6:699], w[ids[6:699].long()].double() * 1.5, U * w[ids[6:699].long()].double().abs() * 1.5)
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids="-".join)
+def test_norm_rows_that_meet_vectors_differently(layers, pair):
+    """Views whose rows start anywhere, alike or not in the matrices of a call."""
+    for n, d, off, pitch in ((3000, 257, 1, 260), (1500, 1001, 3, 1010), (700, 768, 5, 775), (40, 5003, 7, 5013)):
+        wide, _, _ = norm_inputs(n, pitch, pair)
+        x = wide[:, off:off + d]
+        w, b = norm_inputs(1, d, pair)[1:]
+        mean, rstd = check_norm(layers, x, w, b)
+        g = randn(n, pitch, seed=3, dtype=pair[0])
+        check_norm_grad(layers, x, w, g[:, off:off + d], mean, rstd)  # dx contiguous, x and grad alike
+        check_norm_grad(layers, x, w, g[:, :d], mean, rstd)
+        c = x.contiguous()
+        check_norm_grad(layers, c, w, g[:, :d].contiguous(), mean, rstd)  # all alike
+
+
+def test_captured_long_lists(layers):
+    L = abi()
+    for n, rows in ((5000, 3000), (40000, 70000), (350000, 1 << 20)):
+        ids, g = randint(rows, (n,)), randn(n, 16)
+        b = ctypes.c_uint64()
+        check(L.gids_embedding_grad_workspace(n, rows, 16, ctypes.byref(b)))
+        ws = torch.empty(b.value, dtype=torch.uint8, device=DEV)
+        count = torch.zeros(1, dtype=torch.int64, device=DEV)
+        r = torch.full((n,), -9, dtype=torch.int64, device=DEV)
+        v = torch.zeros((n, 16), device=DEV)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            st = torch.cuda.current_stream().cuda_stream
+            dw = layers.embedding_grad(ids, g, rows)
+            check(L.gids_embedding_group(0, ids.data_ptr(), 8, n, rows, -1, 16, ws.data_ptr(), b.value,
+                                         count.data_ptr(), None, st))
+            check(L.gids_embedding_grad_rows(0, r.data_ptr(), v.data_ptr(), 0, 16, n, rows, 16, g.data_ptr(), 0, 16,
+                                             n, 1.0, ws.data_ptr(), b.value, st))
+        for rep in range(3):
+            ids.copy_(randint(rows // (rep + 1), (n,), seed=rep + 1))
+            g.copy_(randn(n, 16, seed=rep + 1))
+            r.fill_(-9)
+            gr.replay()
+            torch.cuda.synchronize()
+            want_r, want_v = layers.embedding_grad_rows(ids, g, rows)
+            k = int(count)
+            assert k == len(want_r) and torch.equal(r[:k], want_r) and bool((r[k:] == -9).all())
+            assert torch.equal(bits(v[:k]), bits(want_v))
+            assert torch.equal(bits(dw), bits(layers.embedding_grad(ids, g, rows)))
+
+
+def test_calls_from_several_threads(layers):
+    import threading
+
+    jobs = []
+    for t in range(4):
+        n = (100, 3000, 40000, 9000)[t]
+        ids, w, g = randint(700, (n,), seed=t), randn(700, 72, seed=t), randn(n, 72, seed=t + 9)
+        want = (layers.embedding(ids, w, scale=0.5), layers.embedding_grad(ids, g, 700), layers.layer_norm(g),
+                *layers.embedding_grad_rows(ids, g, 700))
+        jobs.append((ids, w, g, want))
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(ids, w, g, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = (layers.embedding(ids, w, scale=0.5), layers.embedding_grad(ids, g, 700),
+                           layers.layer_norm(g), *layers.embedding_grad_rows(ids, g, 700))
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(bits(a), bits(b)) for a, b in zip(got, want)):
+                        bad.append("differs")
+        except Exception as e:  # reported by the main thread
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad, bad[:3]
+
+
+def test_counting_rows_in_a_capture_leaves_python_usable(layers):
+    ids, g = randint(50, (300,)), randn(300, 8)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = layers.layer_norm(g)
+        with pytest.raises(RuntimeError, match="captured"):
+            layers.embedding_grad_rows(ids, g, 50)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(bits(y), bits(layers.layer_norm(g)))
+    layers.embedding_grad_rows(ids, g, 50)
