@@ -144,15 +144,26 @@ __global__ void __launch_bounds__(ODD_THREADS) embedding_odd_kernel(EmbArgs a, u
     O* out = reinterpret_cast<O*>(a.out) + (long long)row * a.out_stride + (long long)(unit - row * slabs) * ODD_SLAB;
     const W* in = reinterpret_cast<const W*>(ring + stage * PITCH + (reinterpret_cast<uintptr_t>(src) & 15));
     if (!src && lane == 0) *reinterpret_cast<volatile int*>(a.err) = 1;
-#pragma unroll 4
-    for (int e = (int)lane; e < len; e += 32) {
+    const auto value = [&](int e) -> O {
       if constexpr (std::is_same<W, O>::value) {
-        if (a.scale == 1.0f && src) {  // a copy, NaN bits included
-          out[e] = in[e];
-          continue;
-        }
+        if (a.scale == 1.0f && src) return in[e];  // a copy, NaN bits included
       }
-      out[e] = from_f32<O>(src ? a.scale * to_f32(in[e]) : 0.0f);
+      return from_f32<O>(src ? a.scale * to_f32(in[e]) : 0.0f);
+    };
+    if constexpr (sizeof(O) == 4) {
+#pragma unroll 4
+      for (int e = (int)lane; e < len; e += 32) out[e] = value(e);
+    } else {  // pairs, from the first element on a 4-byte boundary
+      const int head = (reinterpret_cast<uintptr_t>(out) & 2) ? 1 : 0;
+      if (head && lane == 0) out[0] = value(0);
+#pragma unroll 4
+      for (int e = head + 2 * (int)lane; e + 1 < len; e += 64) {
+        RowVec<O, 2> two;
+        two.v[0] = value(e);
+        two.v[1] = value(e + 1);
+        store_raw(out + e, two);
+      }
+      if (((len - head) & 1) && lane == 31) out[len - 1] = value(len - 1);
     }
     stage = stage + 1 == ODD_STAGES ? 0 : stage + 1;
   }
@@ -1047,17 +1058,16 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
     for (int j = 0; j < VEC; j++) f[j] = a.scale * (j & 1 ? acc[j / 2].hi() : acc[j / 2].lo());
     store_vec<W, VEC>(reinterpret_cast<W*>(a.out) + (long long)key * a.out_stride + col, f);
   }
-  float zero[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; j++) zero[j] = 0.0f;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const long long pieces = a.dim * (long long)sizeof(W) / 16;  // (whole: rows are in vectors)
   for (unsigned int row = warp; row < none; row += warps) {
     unsigned int at[WORDS], any = 0;
     lookup(row, at);
 #pragma unroll
     for (int w = 0; w < WORDS; w++) any |= at[w];
     if (any) continue;
-    W* out = reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride;
-    for (long long c = lane * VEC; c < a.dim; c += 32 * VEC) store_vec<W, VEC>(out + c, zero);
+    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride);
+    for (long long c = lane; c < pieces; c += 32) out[c] = zero;
   }
 }
 
@@ -1328,6 +1338,8 @@ void launch_embedding_vec(const EmbArgs& a, const Rows& out, const Rows& weight,
                           cudaStream_t st) {
   constexpr int BIG = 16 / (int)sizeof(W);  // a 16-byte vector of the table
   if (vec_ok(out, dim, BIG) && vec_ok(weight, dim, BIG)) return launch_embedding<W, O, BIG>(a, n, dim, id_bytes, st);
+  if (vec_ok(out, dim, BIG / 2) && vec_ok(weight, dim, BIG / 2))
+    return launch_embedding<W, O, BIG / 2>(a, n, dim, id_bytes, st);
   // a warp to a slab pays off from a few hundred bytes of row on
   if (dim * (int64_t)sizeof(W) < 256) return launch_embedding<W, O, 1>(a, n, dim, id_bytes, st);
   const uint64_t slabs = ((uint64_t)dim + ODD_SLAB - 1) / ODD_SLAB;
