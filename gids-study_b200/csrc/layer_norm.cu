@@ -170,7 +170,10 @@ __device__ __forceinline__ void group_sums(float (&s)[N], int group, int lane, i
 // Rows arrive through a ring in shared memory by asynchronous copies, STAGES - 1
 // iterations ahead of their use. With VEC > 1 a thread copies its own vectors to
 // slots that only it reads, so there is no barrier.
-template <typename X, int VEC, int K, int R, int A, int STAGES, bool FULL, int THREADS, int GROUP>
+// MODE: how a thread's vectors lie to the row. FULL_ROWS: all K are the row's;
+// WHOLE_VECS: each is, or has no column of it (aligned rows); EDGES: any.
+constexpr int EDGES = 0, WHOLE_VECS = 1, FULL_ROWS = 2;
+template <typename X, int VEC, int K, int R, int A, int STAGES, int MODE, int THREADS, int GROUP>
 struct RowRing {
   static constexpr bool STAGED = VEC == 1;
   const RowWalk& walk;
@@ -189,7 +192,7 @@ struct RowRing {
     const long long first = this->first(), block = (long long)blockIdx.x * blockDim.y;
     rows = first < w.n ? (int)((w.n - first + w.total - 1) / w.total) : 0;
     steps = block < w.n ? (int)((w.n - block + w.total - 1) / w.total) : 0;
-    if constexpr (!STAGED && !FULL)
+    if constexpr (!STAGED && MODE == EDGES)
       lead = (int)((reinterpret_cast<uintptr_t>(x) + first * stride * sizeof(X)) & 15) / (int)sizeof(X);
     if constexpr (STAGED)
       mem = static_cast<char*>(dyn) + (size_t)threadIdx.y * STAGES * R * A * pitch(w.dim);
@@ -201,7 +204,11 @@ struct RowRing {
   // first column of vector k; the columns that a thread has of it are in [0, dim)
   __device__ __forceinline__ int col(int k) const { return (k * group + t) * VEC - lead; }
   // whether vector k has elements that are not the row's
-  __device__ __forceinline__ bool partial(int k) const { return !FULL && (col(k) < 0 || col(k) + VEC > walk.dim); }
+  __device__ __forceinline__ bool partial(int k) const {
+    return MODE == EDGES && (col(k) < 0 || col(k) + VEC > walk.dim);
+  }
+  // whether vector k has none that are
+  __device__ __forceinline__ bool absent(int k) const { return MODE != FULL_ROWS && col(k) >= walk.dim; }
   // where this thread starts in a matrix: its first column (STAGED: the row) of the group's first row
   __device__ __forceinline__ char* start(const void* p, long long stride) const {
     return reinterpret_cast<char*>(const_cast<void*>(p)) +
@@ -223,7 +230,7 @@ struct RowRing {
     } else {
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        const bool in = on && (FULL || col(k) < walk.dim);
+        const bool in = on && !absent(k);
         copy_async(slot(ahead, r, k, which), in ? src + k * group * 16 : walk.safe, in);
       }
     }
@@ -270,8 +277,8 @@ struct RowRing {
     float f[K][VEC];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      if (FULL) {
-        load_param<VEC>(p, type, col(k), fill, f[k]);
+      if (MODE != EDGES) {
+        load_param<VEC>(absent(k) ? nullptr : p, type, col(k), fill, f[k]);
       } else {
 #pragma unroll
         for (int j = 0; j < VEC; j++) {
@@ -289,7 +296,9 @@ struct RowRing {
   // vector k of a row of the result (`dst`: start() and jumps)
   __device__ __forceinline__ void store(char* dst, int k, const float (&f)[VEC]) const {
     X* p = reinterpret_cast<X*>(dst) + (STAGED ? col(k) : k * group * VEC);
-    if (!partial(k)) {
+    if (MODE != EDGES) {
+      if (!absent(k)) store_vec<X, VEC>(p, f);
+    } else if (!partial(k)) {
       store_vec<X, VEC>(p, f);
     } else {
 #pragma unroll
@@ -305,9 +314,8 @@ struct RowRing {
 // mean of the differences from it: the second pass takes it out again.
 __device__ __forceinline__ float variance(float mean_sq, float off) { return fmaxf(mean_sq - off * off, 0.0f); }
 
-// blockDim = (threads of a group, groups). FULL: every thread of a group has K
-// whole vectors of each row.
-template <typename X, int VEC, int K, int R, int STAGES, bool FULL, int THREADS, int GROUP>
+// blockDim = (threads of a group, groups).
+template <typename X, int VEC, int K, int R, int STAGES, int MODE, int THREADS, int GROUP>
 __global__ void __launch_bounds__(THREADS) ln_kernel(LnArgs a) {
   extern __shared__ uint4 dyn[];
   constexpr int N = 2 * R, P = VEC * K / 2;
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(THREADS) ln_kernel(LnArgs a) {
   const int group = GROUP ? GROUP : blockDim.x;
   const int lin = threadIdx.y * group + threadIdx.x, lane = lin & 31, warp = lin >> 5;
   int turn = 0;
-  RowRing<X, VEC, K, R, 1, STAGES, FULL, THREADS, GROUP> ring(dyn, a.walk, a.x, a.x_stride);
+  RowRing<X, VEC, K, R, 1, STAGES, MODE, THREADS, GROUP> ring(dyn, a.walk, a.x, a.x_stride);
   const char* xp = ring.start(a.x, a.x_stride);
   char* yp = ring.start(a.y, a.y_stride);
   const auto fetch = [&](int m) {
@@ -356,10 +364,18 @@ __global__ void __launch_bounds__(THREADS) ln_kernel(LnArgs a) {
       F2 d0(0.0f), d1(0.0f);
 #pragma unroll
       for (int p = 0; p < P; p++) f[r][p] = add2(f[r][p], m);
-      if constexpr (!FULL) {  // elements that are not the row's stay zero
+      // elements that are not the row's stay zero
+      if constexpr (VEC == 1) {
 #pragma unroll
-        for (int k = 0; k < K; k++)
-          if (VEC > 1 && ring.partial(k)) {
+        for (int p = 0; p < P; p++)
+          f[r][p] = F2(ring.partial(2 * p) ? 0.0f : f[r][p].lo(), ring.partial(2 * p + 1) ? 0.0f : f[r][p].hi());
+      } else if constexpr (MODE != FULL_ROWS) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+          if (ring.absent(k)) {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2) f[r][(k * VEC + j) / 2] = F2(0.0f);
+          } else if (ring.partial(k)) {
 #pragma unroll
             for (int j = 0; j < VEC; j += 2) {
               F2& c = f[r][(k * VEC + j) / 2];
@@ -367,10 +383,6 @@ __global__ void __launch_bounds__(THREADS) ln_kernel(LnArgs a) {
               c = F2(i >= 0 && i < a.dim ? c.lo() : 0.0f, i + 1 >= 0 && i + 1 < a.dim ? c.hi() : 0.0f);
             }
           }
-        if (VEC == 1) {
-#pragma unroll
-          for (int p = 0; p < P; p++)
-            f[r][p] = F2(ring.partial(2 * p) ? 0.0f : f[r][p].lo(), ring.partial(2 * p + 1) ? 0.0f : f[r][p].hi());
         }
       }
 #pragma unroll
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(LN_LONG_THREADS) ln_long_kernel(LnArgs a) {
 // ------------------------------------------------------------------ backward
 // The rows of a block's groups, with dx, and the block's partial dw and db, laid
 // out as in the forward pass.
-template <typename X, int VEC, int K, int R, int STAGES, bool FULL, int THREADS, int GROUP>
+template <typename X, int VEC, int K, int R, int STAGES, int MODE, int THREADS, int GROUP>
 __global__ void __launch_bounds__(THREADS) ln_grad_kernel(LnGradArgs a) {
   extern __shared__ uint4 dyn[];
   constexpr int N = 2 * R, P = VEC * K / 2;
@@ -490,7 +502,7 @@ __global__ void __launch_bounds__(THREADS) ln_grad_kernel(LnGradArgs a) {
   const int group = GROUP ? GROUP : blockDim.x, groups = blockDim.y;
   const int lin = threadIdx.y * group + threadIdx.x, lane = lin & 31, warp = lin >> 5;
   int turn = 0;
-  RowRing<X, VEC, K, R, 2, STAGES, FULL, THREADS, GROUP> ring(dyn, a.walk, a.x, a.x_stride);
+  RowRing<X, VEC, K, R, 2, STAGES, MODE, THREADS, GROUP> ring(dyn, a.walk, a.x, a.x_stride);
   const char* xp = ring.start(a.x, a.x_stride);
   const char* gp = ring.start(a.g, a.g_stride);
   char* dp = ring.start(a.dx, a.dx_stride);
@@ -592,7 +604,7 @@ __global__ void __launch_bounds__(THREADS) ln_grad_kernel(LnGradArgs a) {
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
         const int c = ring.col(k) + j, p = (k * VEC + j) / 2;
-        if (!FULL && (c < 0 || c >= a.dim)) continue;
+        if (MODE != FULL_ROWS && (c < 0 || c >= a.dim)) continue;
         const float w1 = (k * VEC + j) & 1 ? dw[p].hi() : dw[p].lo();
         const float b1 = (k * VEC + j) & 1 ? db[p].hi() : db[p].lo();
         const float pw = r ? cols[c] : 0.0f, pb = r ? cols[a.dim + c] : 0.0f;
@@ -709,7 +721,7 @@ struct Layout {
 struct Plan {
   int group, groups;
   unsigned int grid;
-  bool full;
+  int mode;
 };
 // Threads of a group when each has k vectors of VEC elements: part of a warp (a
 // power of two) or whole warps; whole warps where the group stages rows.
@@ -739,7 +751,9 @@ Plan plan_of(int64_t n, int dim, int k, int rows, int threads, const Layout& l, 
     while (grid * p.groups % l.period) grid--;
   }
   p.grid = (unsigned int)grid;
-  p.full = VEC > 1 && l.aligned && l.params && (int64_t)p.group * k * VEC == dim;
+  p.mode = VEC == 1 || !l.aligned || !l.params || dim % VEC ? EDGES
+           : (int64_t)p.group * k * VEC == dim              ? FULL_ROWS
+                                                            : WHOLE_VECS;
   return p;
 }
 
@@ -758,10 +772,12 @@ void launch_ln_k(LnArgs a, const Layout& l, int sms, cudaStream_t st) {
   a.walk = walk_of(p, a.n, a.dim, a.x);
   a.x_jump = a.walk.total * a.x_stride * (long long)sizeof(X);
   a.y_jump = a.walk.total * a.y_stride * (long long)sizeof(X);
-  const size_t smem = RowRing<X, VEC, K, R, 1, STAGES, true, LN_THREADS, GROUP>::bytes(p.groups, a.dim);
-  // (plan_of has no full rows of single elements)
-  const auto kernel = p.full ? ln_kernel<X, VEC, K, R, STAGES, (VEC > 1), LN_THREADS, GROUP>
-                             : ln_kernel<X, VEC, K, R, STAGES, false, LN_THREADS, GROUP>;
+  const size_t smem = RowRing<X, VEC, K, R, 1, STAGES, EDGES, LN_THREADS, GROUP>::bytes(p.groups, a.dim);
+  auto kernel = ln_kernel<X, VEC, K, R, STAGES, EDGES, LN_THREADS, GROUP>;
+  if constexpr (VEC > 1) {
+    if (p.mode == FULL_ROWS) kernel = ln_kernel<X, VEC, K, R, STAGES, FULL_ROWS, LN_THREADS, GROUP>;
+    if (p.mode == WHOLE_VECS) kernel = ln_kernel<X, VEC, K, R, STAGES, WHOLE_VECS, LN_THREADS, GROUP>;
+  }
   if (smem > 40 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<p.grid, dim3(p.group, p.groups), smem, st>>>(a);
 }
@@ -796,10 +812,13 @@ int launch_ln_grad_k(LnGradArgs a, const Layout& l, int sms, cudaStream_t st) {
   a.x_jump = a.walk.total * a.x_stride * (long long)sizeof(X);
   a.g_jump = a.walk.total * a.g_stride * (long long)sizeof(X);
   a.dx_jump = a.walk.total * a.dx_stride * (long long)sizeof(X);
-  const size_t smem = std::max(RowRing<X, VEC, K, R, 2, STAGES, true, LN_THREADS, GROUP>::bytes(p.groups, a.dim),
+  const size_t smem = std::max(RowRing<X, VEC, K, R, 2, STAGES, EDGES, LN_THREADS, GROUP>::bytes(p.groups, a.dim),
                                p.groups > 1 ? (size_t)a.dim * 2 * sizeof(float) : 0);
-  const auto kernel = p.full ? ln_grad_kernel<X, VEC, K, R, STAGES, (VEC > 1), LN_THREADS, GROUP>
-                             : ln_grad_kernel<X, VEC, K, R, STAGES, false, LN_THREADS, GROUP>;
+  auto kernel = ln_grad_kernel<X, VEC, K, R, STAGES, EDGES, LN_THREADS, GROUP>;
+  if constexpr (VEC > 1) {
+    if (p.mode == FULL_ROWS) kernel = ln_grad_kernel<X, VEC, K, R, STAGES, FULL_ROWS, LN_THREADS, GROUP>;
+    if (p.mode == WHOLE_VECS) kernel = ln_grad_kernel<X, VEC, K, R, STAGES, WHOLE_VECS, LN_THREADS, GROUP>;
+  }
   if (smem > 40 * 1024) allow_smem(reinterpret_cast<const void*>(kernel), smem);
   kernel<<<p.grid, dim3(p.group, p.groups), smem, st>>>(a);
   return (int)p.grid;
