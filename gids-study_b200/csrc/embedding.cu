@@ -211,13 +211,18 @@ __device__ __forceinline__ unsigned long long source_word(const IdSource& s, uns
 // Zeros for the rows of a dense gradient, written while the sort leaves the
 // memory idle: every kernel of the sort takes a share, as bulk copies of a zero
 // block of shared memory that run beside its own work. `bytes` and the
-// address are multiples of 16.
+// address are multiples of 16; `tail` bytes more (a multiple of 2) follow.
 constexpr int ZERO_BYTES = 8192;
 struct ZeroFill {
   char* p;
   unsigned long long bytes;
+  unsigned int tail;
 };
+__device__ __forceinline__ void zero_tail(const ZeroFill& z) {
+  if (blockIdx.x == 0 && threadIdx.x < z.tail / 2) reinterpret_cast<unsigned short*>(z.p + z.bytes)[threadIdx.x] = 0;
+}
 __device__ __forceinline__ void zero_begin(const ZeroFill& z, uint4* zeros) {
+  zero_tail(z);
   if (!z.bytes) return;
   for (int i = threadIdx.x; i < ZERO_BYTES / 16; i += blockDim.x) zeros[i] = make_uint4(0, 0, 0, 0);
   // the copies read shared memory through the asynchronous proxy
@@ -276,11 +281,11 @@ __global__ void __launch_bounds__(THREADS) count_kernel(IdSource src, Pass p, Ze
 
 template <int THREADS>
 struct SortShared {
-  unsigned int base[MAX_RADIX];                  // next output index of each digit
-  unsigned int before[MAX_RADIX];                // words of the digit in earlier tiles
-  unsigned short wcount[(THREADS / 32)][MAX_RADIX];  // digits of this step, by warp
+  unsigned int base[MAX_RADIX];                    // next output index of each digit
+  unsigned int before[MAX_RADIX];                  // words of the digit in earlier tiles
+  unsigned short wcount[THREADS / 32][MAX_RADIX];  // digits of this step, by warp
   unsigned short part[4][MAX_RADIX];
-  unsigned int wsum[(THREADS / 32)];
+  unsigned int wsum[THREADS / 32];
 };
 
 // base[d] = (words of smaller digits) + s.before[d], where thread d < radix
@@ -505,7 +510,7 @@ __global__ void __launch_bounds__(THREADS) head_rank_kernel(const unsigned long 
                                                                  unsigned int* __restrict__ rank,
                                                                  unsigned long long* count,
                                                                  volatile unsigned long long* host_count) {
-  __shared__ unsigned int wsum[(THREADS / 32)];
+  __shared__ unsigned int wsum[THREADS / 32];
   __shared__ unsigned int heads;
   chain_wait();
   if (threadIdx.x == 0) heads = 0;
@@ -662,6 +667,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) cluster_sort_kernel(IdSource 
 // in the chain finds both done.
 __global__ void __launch_bounds__(256) zero_kernel(ZeroFill z) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  zero_tail(z);
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (unsigned long long at = ((unsigned long long)blockIdx.x * 256 + threadIdx.x) * 16; at < z.bytes;
        at += (unsigned long long)gridDim.x * 256 * 16)
@@ -767,11 +773,12 @@ __global__ void __launch_bounds__(SEG_THREADS, 4) segment_kernel(SegArgs a) {
   const unsigned int b0 = block * rows;  // < n
   const unsigned int here = min(rows, a.n - b0);
   chain_wait();
-  // words[1 + i] is word b0 + i; a word without a row gets the key NONE
+  // words[1 + i] is word b0 + i; a word without a row gets the key NONE (and one
+  // of another call's list, whose position is not one of this gradient)
   for (unsigned int i = threadIdx.x; i < rows + 2; i += SEG_THREADS) {
     const bool in = i <= here + 1 && (i > 0 || b0 > 0) && (i <= here || b0 + here < a.n);
     const unsigned long long w = in ? a.words[b0 + i - 1] : ~0ull;
-    words[i] = (unsigned int)(w >> 32) < a.num_rows ? w : ~0ull;
+    words[i] = (unsigned int)(w >> 32) < a.num_rows && (unsigned int)w < a.n ? w : ~0ull;
   }
   __syncthreads();
   const Columns<VEC, K> c(a, slab);
@@ -973,9 +980,9 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
 #pragma unroll
     for (int w = 0; w < WORDS; w++) at[w] = __ballot_sync(0xffffffffu, mine[w] == key);
   };
-  for (unsigned int task = warp; task < a.n * a.slabs; task += warps) {
-    const unsigned int i = task / a.slabs;
-    const long long col = ((long long)(task - i * a.slabs) * 32 + lane) * VEC;
+  for (unsigned long long task = warp; task < (unsigned long long)a.n * a.slabs; task += warps) {
+    const unsigned int i = (unsigned int)(task / a.slabs);
+    const long long col = ((long long)(task - (unsigned long long)i * a.slabs) * 32 + lane) * VEC;
     const unsigned int key = keys[i];
     unsigned int at[WORDS];
     lookup(key, at);
@@ -1060,9 +1067,9 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
   }
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const long long pieces = a.dim * (long long)sizeof(W) / 16;  // (whole: rows are in vectors)
-  for (unsigned int row = warp; row < none; row += warps) {
+  for (unsigned long long row = warp; row < none; row += warps) {  // (none may be close to 2^32)
     unsigned int at[WORDS], any = 0;
-    lookup(row, at);
+    lookup((unsigned int)row, at);
 #pragma unroll
     for (int w = 0; w < WORDS; w++) any |= at[w];
     if (any) continue;
@@ -1210,7 +1217,7 @@ void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay
     chain(true, cluster_sort_kernel, blocks, CLUSTER_THREADS, sizeof(ClusterShared), st, Cluster{blocks}, ids,
           (unsigned int)n, key_bits_of(ids.num_rows), (int)items, blocks,
           reinterpret_cast<unsigned long long*>(ws + lay.words_a), ranks ? rank : nullptr, count, host_count);
-    if (zero.bytes) chain(false, zero_kernel, (unsigned int)sms * 4, 256, 0, st, zero);
+    if (zero.bytes || zero.tail) chain(false, zero_kernel, (unsigned int)sms * 4, 256, 0, st, zero);
     return;
   }
   unsigned int tiles, per;
@@ -1222,9 +1229,10 @@ void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay
   // an equal share of the zeros to every kernel
   const uint64_t share = (zero.bytes / (2 * passes) + 15) / 16 * 16;
   const auto next_share = [&] {
-    const ZeroFill z{zero.p, std::min<uint64_t>(share, zero.bytes)};
+    ZeroFill z{zero.p, std::min<uint64_t>(share, zero.bytes), 0};
     zero.p += z.bytes;
     zero.bytes -= z.bytes;
+    if (!zero.bytes) std::swap(z.tail, zero.tail);  // the last share
     return z;
   };
   IdSource src = ids;
@@ -1299,7 +1307,6 @@ template <typename G, typename W>
 void launch_tiny(TinyArgs a, int sms, cudaStream_t st) {
   constexpr int VEC = 16 / (int)sizeof(G);
   a.slabs = (unsigned int)((a.dim + 32 * VEC - 1) / (32 * VEC));
-  GIDS_CHECK((uint64_t)a.n * a.slabs < (1ull << 32), GIDS_E_UNSUPPORTED, "too many columns");
   const SegPlan plan = seg_plan(a.n, (uint64_t)a.dim, sizeof(G));
   a.chunk = plan.chunk;
   a.rows = plan.rows;
@@ -1501,13 +1508,15 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
   }
   const size_t eb = (size_t)type_bytes(dweight.type);
   const uint64_t total = (uint64_t)num_rows * (uint64_t)dim * eb;
-  ZeroFill zero{static_cast<char*>(dweight.p), total};
-  // the zeros go out beside the sort if they are one aligned stretch of memory
-  if (n == 0 || (num_rows > 1 && dweight.stride != dim) || ((uintptr_t)dweight.p) % 16 || total % 16) {
-    zero.bytes = 0;
-    if (num_rows > 0)
-      GIDS_CUDA(cudaMemset2DAsync(dweight.p, (num_rows > 1 ? (size_t)dweight.stride : (size_t)dim) * eb, 0,
-                                  (size_t)dim * eb, (size_t)num_rows, st));
+  ZeroFill zero{static_cast<char*>(dweight.p), total / 16 * 16, (unsigned int)(total % 16)};
+  // the zeros go out beside the sort if they are one stretch of memory
+  const bool stretch = num_rows <= 1 || dweight.stride == dim;
+  if (n == 0 || !stretch || ((uintptr_t)dweight.p) % 16) {
+    zero = ZeroFill{};
+    if (stretch)
+      GIDS_CUDA(cudaMemsetAsync(dweight.p, 0, total, st));
+    else
+      GIDS_CUDA(cudaMemset2DAsync(dweight.p, (size_t)dweight.stride * eb, 0, (size_t)dim * eb, (size_t)num_rows, st));
   }
   if (n == 0) return;
   char* base = static_cast<char*>(ws);
@@ -1555,7 +1564,7 @@ void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64
   unsigned long long* count =
       count_dev ? reinterpret_cast<unsigned long long*>(count_dev) : reinterpret_cast<unsigned long long*>(base + lay.count);
   sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay,
-           ZeroFill{nullptr, 0}, true, count, word.dev, 1, st);
+           ZeroFill{}, true, count, word.dev, 1, st);
   if (count_host) {
     GIDS_CUDA(cudaStreamSynchronize(st));
     *count_host = *reinterpret_cast<volatile unsigned long long*>(word.host);
@@ -1599,6 +1608,10 @@ void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacit
 void embedding_check(int device, cudaStream_t st) {
   check_device(device);
   DeviceGuard dg(device);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  GIDS_CUDA(cudaStreamIsCapturing(st, &cap));
+  GIDS_CHECK(cap == cudaStreamCaptureStatusNone, GIDS_E_STATE,
+             "the check waits for the stream, which is being captured into a graph");
   GIDS_CUDA(cudaStreamSynchronize(st));
   check_id_errors(device);
 }

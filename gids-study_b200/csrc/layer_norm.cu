@@ -899,7 +899,7 @@ template <typename X>
 void ln_typed(const LnArgs& a, const Layout& l, int sms, cudaStream_t st) {
   constexpr int BIG = 16 / (int)sizeof(X);
   const unsigned int long_grid = (unsigned int)std::min<int64_t>(a.n, (int64_t)sms * 4);
-  if (l.alike && group_of<BIG>(a.dim, 32 / BIG, l) <= LN_THREADS)
+  if (l.alike && l.period <= sms && group_of<BIG>(a.dim, 32 / BIG, l) <= LN_THREADS)
     launch_ln<X, BIG>(a, l, sms, st);
   else if (group_of<1>(a.dim, 32, l) <= LN_THREADS)
     launch_ln<X, 1>(a, l, sms, st);
@@ -914,7 +914,7 @@ template <typename X>
 void ln_grad_typed(const LnGradArgs& a, const Layout& l, int p_type, void* dw, void* db, int sms, cudaStream_t st) {
   constexpr int BIG = 16 / (int)sizeof(X);
   int parts;
-  if (l.alike && group_of<BIG>(a.dim, 4, l) <= LN_THREADS)
+  if (l.alike && l.period <= sms && group_of<BIG>(a.dim, 4, l) <= LN_THREADS)
     parts = launch_ln_grad<X, BIG>(a, l, sms, st);
   else if (group_of<1>(a.dim, 4 * BIG, l) <= LN_THREADS)
     parts = launch_ln_grad<X, 1>(a, l, sms, st);
@@ -946,6 +946,8 @@ void layer_norm(int device, Rows y, float* mean, float* rstd, Rows x, const void
   check_param(weight, param_type, "weight");
   check_param(bias, param_type, "bias");
   GIDS_CHECK((mean == nullptr) == (rstd == nullptr), GIDS_E_INVAL, "mean and rstd come together or not at all");
+  check_param(mean, GIDS_F32, "mean");
+  check_param(rstd, GIDS_F32, "rstd");
   GIDS_CHECK(eps >= 0.0f, GIDS_E_INVAL, "eps must be >= 0");
   if (n == 0) return;
   DeviceGuard dg(device);
@@ -991,6 +993,8 @@ void layer_norm_grad(int device, Rows dx, void* dweight, void* dbias, Rows grad,
   check_param(dweight, param_type, "dweight");
   check_param(dbias, param_type, "dbias");
   GIDS_CHECK(n == 0 || (mean && rstd), GIDS_E_INVAL, "mean or rstd is null");
+  check_param(mean, GIDS_F32, "mean");
+  check_param(rstd, GIDS_F32, "rstd");
   const bool params = dweight || dbias;
   if (params && n) {
     GIDS_CHECK(ws && ((uintptr_t)ws) % 256 == 0, GIDS_E_INVAL, "workspace is null or not aligned to 256 bytes");

@@ -841,3 +841,55 @@ def test_counting_rows_in_a_capture_leaves_python_usable(layers):
     torch.cuda.synchronize()
     assert torch.equal(bits(y), bits(layers.layer_norm(g)))
     layers.embedding_grad_rows(ids, g, 50)
+
+
+def test_rows_of_another_list_stay_inside_the_gradient(layers):
+    """gids_embedding_grad_rows after gids_embedding_group of fewer ids, on the same
+    workspace: the call's own bounds hold, whatever the words say."""
+    L = abi()
+    g = randn(3000, 8)
+    b = ctypes.c_uint64()
+    check(L.gids_embedding_grad_workspace(3000, 50, 8, ctypes.byref(b)))
+    ws = torch.full((b.value,), 0x11, dtype=torch.uint8, device=DEV)
+    ids = randint(50, (100,))
+    count = torch.zeros(1, dtype=torch.int64, device=DEV)
+    check(L.gids_embedding_group(0, ids.data_ptr(), 8, 100, 50, -1, 8, ws.data_ptr(), b.value, count.data_ptr(), None,
+                                 None))
+    r = torch.full((60,), -9, dtype=torch.int64, device=DEV)
+    v = torch.full((60, 8), 7.0, device=DEV)
+    check(L.gids_embedding_grad_rows(0, r.data_ptr(), v.data_ptr(), 0, 8, 40, 50, 8, g.data_ptr(), 0, 8, 3000, 1.0,
+                                     ws.data_ptr(), b.value, None))
+    torch.cuda.synchronize()
+    assert bool((r[40:] == -9).all()) and bool((v[40:] == 7).all())
+
+
+@pytest.mark.parametrize("rows,dim", [(33, 7), (1, 3), (5, 1), (1001, 129)])
+def test_grad_tables_of_odd_size(layers, rows, dim):
+    for n in (5, 300, 40000):
+        for t in ("f32", "f16"):
+            ids, g = randint(max(1, rows // 2), (n,)), randn(n, dim, dtype=t)
+            big = torch.full((rows * dim + 8,), 5.0, device=DEV, dtype=TYPES[t])
+            dw = layers.embedding_grad(ids, g, rows)
+            L = abi()
+            b = ctypes.c_uint64()
+            check(L.gids_embedding_grad_workspace(n, rows, dim, ctypes.byref(b)))
+            ws = torch.empty(b.value, dtype=torch.uint8, device=DEV)
+            check(L.gids_embedding_grad(0, big.data_ptr(), CODES[big.dtype], dim, rows, dim, g.data_ptr(),
+                                        CODES[g.dtype], dim, ids.data_ptr(), 8, n, -1, 1.0, ws.data_ptr(), b.value,
+                                        None))
+            torch.cuda.synchronize()
+            assert torch.equal(bits(big[:rows * dim].view(rows, dim)), bits(dw))
+            assert bool((big[rows * dim:] == 5).all())
+            check_grad(layers, ids, g, rows)
+
+
+def test_checking_ids_in_a_capture_is_refused(layers):
+    g = randn(30, 8)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = layers.layer_norm(g)
+        assert abi().gids_embedding_check(0, torch.cuda.current_stream().cuda_stream) == GIDS_E_STATE
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(bits(y), bits(layers.layer_norm(g)))
