@@ -615,6 +615,19 @@ int gids_embedding_grad_rows(int device, int64_t* rows, void* values, int value_
   });
 }
 
+int gids_embedding_grad_distinct(int device, int64_t* rows, void* values, int value_type, int64_t values_stride,
+                                 int64_t capacity, int64_t num_rows, int64_t dim, const void* grad, int grad_type,
+                                 int64_t grad_stride, const void* ids, int id_bytes, int64_t n, int64_t padding_idx,
+                                 float scale, void* workspace, uint64_t workspace_bytes, uint64_t* count_host,
+                                 void* stream) {
+  return guarded([&] {
+    NEED(count_host);
+    gids::embedding_grad_distinct(device, rows, {values, value_type, values_stride}, capacity, num_rows, dim,
+                                  {const_cast<void*>(grad), grad_type, grad_stride}, ids, id_bytes, n, padding_idx,
+                                  scale, workspace, workspace_bytes, count_host, (cudaStream_t)stream);
+  });
+}
+
 int gids_layer_norm(int device, void* y, int64_t y_stride, float* mean, float* rstd, const void* x, int x_type,
                     int64_t x_stride, const void* weight, const void* bias, int param_type, int64_t n, int64_t dim,
                     float eps, void* stream) {

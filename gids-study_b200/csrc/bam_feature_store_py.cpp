@@ -527,6 +527,24 @@ PYBIND11_MODULE(BAM_Feature_Store, m) {
       py::arg("capacity"), py::arg("num_rows"), py::arg("dim"), py::arg("grad"), py::arg("grad_type"),
       py::arg("grad_stride"), py::arg("n"), py::arg("scale"), py::arg("workspace"), py::arg("workspace_bytes"),
       py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
+  // both in one call; returns the number of distinct rows (waits for the stream)
+  m.def(
+      "embedding_grad_distinct",
+      [](int device, uint64_t rows, uint64_t values, int value_type, int64_t values_stride, int64_t capacity,
+         int64_t num_rows, int64_t dim, uint64_t grad, int grad_type, int64_t grad_stride, uint64_t ids, int id_bytes,
+         int64_t n, int64_t padding_idx, float scale, uint64_t workspace, uint64_t workspace_bytes, uint64_t stream) {
+        uint64_t count = 0;
+        check(gids_embedding_grad_distinct(device, (int64_t*)rows, (void*)values, value_type, values_stride, capacity,
+                                           num_rows, dim, (const void*)grad, grad_type, grad_stride, (const void*)ids,
+                                           id_bytes, n, padding_idx, scale, (void*)workspace, workspace_bytes, &count,
+                                           (void*)stream));
+        return count;
+      },
+      py::arg("device"), py::arg("rows"), py::arg("values"), py::arg("value_type"), py::arg("values_stride"),
+      py::arg("capacity"), py::arg("num_rows"), py::arg("dim"), py::arg("grad"), py::arg("grad_type"),
+      py::arg("grad_stride"), py::arg("ids"), py::arg("id_bytes"), py::arg("n"), py::arg("padding_idx"),
+      py::arg("scale"), py::arg("workspace"), py::arg("workspace_bytes"), py::arg("stream") = 0,
+      py::call_guard<py::gil_scoped_release>());
   m.def(
       "layer_norm",
       [](int device, uint64_t y, int64_t y_stride, uint64_t mean, uint64_t rstd, uint64_t x, int x_type,

@@ -943,10 +943,11 @@ __global__ void __launch_bounds__(SEG_THREADS) join_kernel(SegArgs a) {
   store_result<W, VEC, K>(a, c, cur, b1 - 1, acc);
 }
 
-// A dense gradient of a few ids in one kernel: every warp looks for its ids in
-// the whole list instead of in a sorted one. A warp takes an id's first position
-// and a slab of columns and adds the rows of the positions that share the id;
-// and it zeroes table rows that no id names. The additions are those of
+// The gradient of a few ids in one kernel: every warp looks for its ids in the
+// whole list instead of in a sorted one. A warp takes an id's first position and
+// a slab of columns and adds the rows of the positions that share the id. Dense:
+// it also zeroes table rows that no id names. Distinct rows (rows_out): an id's
+// row is the number of smaller ids. The additions are those of
 // segment_kernel and join_kernel, chunk by chunk and block by block of the
 // sorted list, so that the dense form and the distinct rows hold the same bits.
 constexpr unsigned int TINY_IDS = 128;
@@ -960,6 +961,9 @@ struct TinyArgs {
   unsigned int n, slabs;
   unsigned int chunk, rows;  // words of a chunk and of a block (powers of two)
   float scale;
+  long long* rows_out;  // null: dense
+  unsigned int capacity;
+  volatile unsigned long long* host_count;  // with rows_out: how many
 };
 
 template <typename G, typename W, int VEC>
@@ -974,8 +978,20 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
   const unsigned int warp = blockIdx.x * (TINY_THREADS / 32) + (threadIdx.x >> 5);
   const unsigned int warps = gridDim.x * (TINY_THREADS / 32);
   unsigned int mine[WORDS];
+  bool lead[WORDS];  // first of its id
 #pragma unroll
-  for (int w = 0; w < WORDS; w++) mine[w] = keys[w * 32 + lane];
+  for (int w = 0; w < WORDS; w++) {
+    mine[w] = keys[w * 32 + lane];
+    lead[w] = mine[w] != none;
+    if (a.rows_out)
+      for (unsigned int j = 0; j < w * 32 + lane; j++) lead[w] = lead[w] && keys[j] != mine[w];
+  }
+  if (a.rows_out && blockIdx.x == 0 && threadIdx.x < 32) {
+    unsigned int all = 0;
+#pragma unroll
+    for (int w = 0; w < WORDS; w++) all += __popc(__ballot_sync(0xffffffffu, lead[w]));
+    if (threadIdx.x == 0) *a.host_count = all;
+  }
   const auto lookup = [&](unsigned int key, unsigned int (&at)[WORDS]) {  // the positions of `key`
 #pragma unroll
     for (int w = 0; w < WORDS; w++) at[w] = __ballot_sync(0xffffffffu, mine[w] == key);
@@ -986,14 +1002,17 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
     const unsigned int key = keys[i];
     unsigned int at[WORDS];
     lookup(key, at);
-    unsigned int first = TINY_IDS, left = 0, index = 0;  // index: where the id's run starts in the sorted list
+    // index: where the id's run starts in the sorted list; row: of the result
+    unsigned int first = TINY_IDS, left = 0, index = 0, row = a.rows_out ? 0 : key;
 #pragma unroll
     for (int w = WORDS - 1; w >= 0; w--) {
       if (at[w]) first = w * 32 + __ffs(at[w]) - 1;
       left += __popc(at[w]);
       index += __popc(__ballot_sync(0xffffffffu, mine[w] < key));
+      if (a.rows_out) row += __popc(__ballot_sync(0xffffffffu, lead[w] && mine[w] < key));
     }
-    if (key == none || first != i || col >= a.dim) continue;  // (no shuffles below)
+    if (key == none || first != i || col >= a.dim || row >= a.capacity) continue;  // (no shuffles below)
+    if (a.rows_out && col == 0) a.rows_out[row] = (long long)key;
     // sums of the chunk, of the block up to the chunk, of the run up to the block
     F2 acc[P], blk[P], tot[P];
     bool in_blk = false, in_tot = false;
@@ -1063,8 +1082,9 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
     float f[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; j++) f[j] = a.scale * (j & 1 ? acc[j / 2].hi() : acc[j / 2].lo());
-    store_vec<W, VEC>(reinterpret_cast<W*>(a.out) + (long long)key * a.out_stride + col, f);
+    store_vec<W, VEC>(reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride + col, f);
   }
+  if (a.rows_out) return;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const long long pieces = a.dim * (long long)sizeof(W) / 16;  // (whole: rows are in vectors)
   for (unsigned long long row = warp; row < none; row += warps) {  // (none may be close to 2^32)
@@ -1296,8 +1316,8 @@ void segments(const SegArgs& a, const Rows& out, const Rows& grad, bool first, c
   return launch_segments_vec<__nv_bfloat16, __nv_bfloat16>(a, out, grad, first, st);
 }
 
-// Whether a dense gradient goes to tiny_grad_kernel: few ids, rows in vectors.
-// (64 ids into 5,000 x 128 fp32: 16 us a pass, 10 in one kernel.)
+// Whether a gradient goes to tiny_grad_kernel: few ids, rows in vectors. (64 ids
+// into 5,000 x 128 fp32, dense: 16 us a pass by the sorted list, 12 this way.)
 bool tiny_grad(int64_t n, int64_t dim, const Rows& out, const Rows& grad) {
   const int vec = 16 / type_bytes(grad.type);
   return n <= (int64_t)TINY_IDS && vec_ok(out, dim, vec) && vec_ok(grad, dim, vec);
@@ -1310,7 +1330,7 @@ void launch_tiny(TinyArgs a, int sms, cudaStream_t st) {
   const SegPlan plan = seg_plan(a.n, (uint64_t)a.dim, sizeof(G));
   a.chunk = plan.chunk;
   a.rows = plan.rows;
-  const uint64_t tasks = std::max<uint64_t>((uint64_t)a.n * a.slabs, a.src.num_rows);
+  const uint64_t tasks = std::max<uint64_t>((uint64_t)a.n * a.slabs, a.rows_out ? 0 : a.src.num_rows);
   const unsigned int grid = (unsigned int)std::min<uint64_t>((tasks + 7) / 8, (uint64_t)sms * 8);
   tiny_grad_kernel<G, W, VEC><<<grid, TINY_THREADS, 0, st>>>(a);
   GIDS_CUDA(cudaGetLastError());
@@ -1379,6 +1399,10 @@ struct HostWord {
     if (!host)
       GIDS_CUDA(cudaHostAlloc(&host, sizeof(*host), cudaHostAllocMapped | cudaHostAllocPortable));
     GIDS_CUDA(cudaHostGetDevicePointer(&dev, host, 0));
+  }
+  unsigned long long wait(cudaStream_t st) {
+    GIDS_CUDA(cudaStreamSynchronize(st));
+    return *reinterpret_cast<volatile unsigned long long*>(host);
   }
   ~HostWord() {
     if (!host) return;
@@ -1504,6 +1528,7 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
     t.dim = dim;
     t.n = (unsigned int)n;
     t.scale = scale;
+    t.capacity = (unsigned int)num_rows;
     return tiny(t, dweight, grad, device_sms(device), st);
   }
   const size_t eb = (size_t)type_bytes(dweight.type);
@@ -1537,44 +1562,24 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
   segments(a, dweight, grad, false, st);
 }
 
-void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
-                     int64_t dim, void* ws, uint64_t ws_bytes, uint64_t* count_dev, uint64_t* count_host,
-                     cudaStream_t st) {
+namespace {
+// Checks of the calls that return the number of distinct rows to the host.
+void check_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
+                 int64_t dim, const void* ws, uint64_t ws_bytes) {
   check_device(device);
   check_ids(ids, id_bytes, n, num_rows, dim);
   GIDS_CHECK(padding_idx >= -1 && padding_idx < std::max<int64_t>(num_rows, 1), GIDS_E_INVAL,
              "padding_idx must be -1 (none) or a row");
-  const Workspace lay((uint64_t)n, (uint64_t)dim);
-  check_workspace(ws, ws_bytes, lay);
-  check_id_errors(device);
-  DeviceGuard dg(device);
-  if (count_host) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    GIDS_CUDA(cudaStreamIsCapturing(st, &cap));
-    GIDS_CHECK(cap == cudaStreamCaptureStatusNone, GIDS_E_STATE,
-               "count_host waits for the stream, which is being captured into a graph");
-  }
-  char* base = static_cast<char*>(ws);
-  if (n == 0) {
-    if (count_dev) GIDS_CUDA(cudaMemsetAsync(count_dev, 0, sizeof(*count_dev), st));
-    if (count_host) *count_host = 0;
-    return;
-  }
-  HostWord word(count_host != nullptr);
-  unsigned long long* count =
-      count_dev ? reinterpret_cast<unsigned long long*>(count_dev) : reinterpret_cast<unsigned long long*>(base + lay.count);
-  sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay,
-           ZeroFill{}, true, count, word.dev, 1, st);
-  if (count_host) {
-    GIDS_CUDA(cudaStreamSynchronize(st));
-    *count_host = *reinterpret_cast<volatile unsigned long long*>(word.host);
-  }
+  check_workspace(ws, ws_bytes, Workspace((uint64_t)n, (uint64_t)dim));
 }
-
-void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacity, int64_t num_rows, int64_t dim,
-                         Rows grad, int64_t n, float scale, void* ws, uint64_t ws_bytes, cudaStream_t st) {
-  check_device(device);
-  check_ids(reinterpret_cast<const void*>(256), 8, n, num_rows, dim);
+void check_not_capturing(cudaStream_t st) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  GIDS_CUDA(cudaStreamIsCapturing(st, &cap));
+  GIDS_CHECK(cap == cudaStreamCaptureStatusNone, GIDS_E_STATE,
+             "count_host waits for the stream, which is being captured into a graph");
+}
+void check_values(const int64_t* rows, const Rows& values, int64_t capacity, const Rows& grad, int64_t n,
+                  int64_t dim) {
   GIDS_CHECK(capacity >= 0, GIDS_E_INVAL, "capacity must be >= 0");
   GIDS_CHECK(capacity == 0 || rows, GIDS_E_INVAL, "rows is null");
   GIDS_CHECK(((uintptr_t)rows) % 8 == 0, GIDS_E_INVAL, "rows: address not aligned to its elements");
@@ -1582,11 +1587,10 @@ void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacit
   check_rows(grad, "grad", n, dim, false);
   GIDS_CHECK(values.type == grad.type || values.type == GIDS_F32, GIDS_E_UNSUPPORTED,
              "values must have the gradient's type or be float32");
-  const Workspace lay((uint64_t)n, (uint64_t)dim);
-  check_workspace(ws, ws_bytes, lay);
-  if (n == 0 || capacity == 0) return;
-  DeviceGuard dg(device);
-  char* base = static_cast<char*>(ws);
+}
+// the sums of the sorted words in the workspace
+void sum_rows(int64_t* rows, const Rows& values, int64_t capacity, int64_t num_rows, int64_t dim, const Rows& grad,
+              int64_t n, float scale, char* base, const Workspace& lay, bool first, cudaStream_t st) {
   SegArgs a{};
   a.words = reinterpret_cast<const unsigned long long*>(base + sorted_at((uint64_t)n, (uint64_t)num_rows, lay));
   a.rank = reinterpret_cast<const unsigned int*>(base + lay.rank);
@@ -1602,7 +1606,79 @@ void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacit
   a.dim = dim;
   a.n = (unsigned int)n;
   a.scale = scale;
-  segments(a, values, grad, true, st);
+  segments(a, values, grad, first, st);
+}
+}  // namespace
+
+void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
+                     int64_t dim, void* ws, uint64_t ws_bytes, uint64_t* count_dev, uint64_t* count_host,
+                     cudaStream_t st) {
+  check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes);
+  check_id_errors(device);
+  DeviceGuard dg(device);
+  if (count_host) check_not_capturing(st);
+  if (n == 0) {
+    if (count_dev) GIDS_CUDA(cudaMemsetAsync(count_dev, 0, sizeof(*count_dev), st));
+    if (count_host) *count_host = 0;
+    return;
+  }
+  const Workspace lay((uint64_t)n, (uint64_t)dim);
+  char* base = static_cast<char*>(ws);
+  HostWord word(count_host != nullptr);
+  unsigned long long* count =
+      count_dev ? reinterpret_cast<unsigned long long*>(count_dev) : reinterpret_cast<unsigned long long*>(base + lay.count);
+  sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, ZeroFill{},
+           true, count, word.dev, 1, st);
+  if (count_host) *count_host = word.wait(st);
+}
+
+void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacity, int64_t num_rows, int64_t dim,
+                         Rows grad, int64_t n, float scale, void* ws, uint64_t ws_bytes, cudaStream_t st) {
+  check_device(device);
+  check_ids(reinterpret_cast<const void*>(256), 8, n, num_rows, dim);
+  check_values(rows, values, capacity, grad, n, dim);
+  const Workspace lay((uint64_t)n, (uint64_t)dim);
+  check_workspace(ws, ws_bytes, lay);
+  if (n == 0 || capacity == 0) return;
+  DeviceGuard dg(device);
+  sum_rows(rows, values, capacity, num_rows, dim, grad, n, scale, static_cast<char*>(ws), lay, true, st);
+}
+
+void embedding_grad_distinct(int device, int64_t* rows, Rows values, int64_t capacity, int64_t num_rows, int64_t dim,
+                             Rows grad, const void* ids, int id_bytes, int64_t n, int64_t padding_idx, float scale,
+                             void* ws, uint64_t ws_bytes, uint64_t* count_host, cudaStream_t st) {
+  check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes);
+  check_values(rows, values, capacity, grad, n, dim);
+  GIDS_CHECK(capacity >= std::min(n, num_rows), GIDS_E_INVAL, "capacity must be at least min(n, num_rows)");
+  check_id_errors(device);
+  DeviceGuard dg(device);
+  check_not_capturing(st);
+  *count_host = 0;
+  if (n == 0) return;
+  const Workspace lay((uint64_t)n, (uint64_t)dim);
+  char* base = static_cast<char*>(ws);
+  HostWord word(true);
+  if (tiny_grad(n, dim, values, grad) && capacity) {
+    TinyArgs t{};
+    t.src = id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device));
+    t.out = values.p;
+    t.grad = grad.p;
+    t.out_stride = values.stride;
+    t.grad_stride = grad.stride;
+    t.dim = dim;
+    t.n = (unsigned int)n;
+    t.scale = scale;
+    t.rows_out = reinterpret_cast<long long*>(rows);
+    t.capacity = (unsigned int)std::min<int64_t>(capacity, n);
+    t.host_count = word.dev;
+    tiny(t, values, grad, device_sms(device), st);
+    *count_host = word.wait(st);
+    return;
+  }
+  sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, ZeroFill{},
+           true, reinterpret_cast<unsigned long long*>(base + lay.count), word.dev, 1, st);
+  if (capacity) sum_rows(rows, values, capacity, num_rows, dim, grad, n, scale, base, lay, false, st);
+  *count_host = word.wait(st);
 }
 
 void embedding_check(int device, cudaStream_t st) {

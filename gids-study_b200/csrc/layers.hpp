@@ -38,6 +38,9 @@ void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64
                      cudaStream_t st);
 void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacity, int64_t num_rows, int64_t dim,
                          Rows grad, int64_t n, float scale, void* ws, uint64_t ws_bytes, cudaStream_t st);
+void embedding_grad_distinct(int device, int64_t* rows, Rows values, int64_t capacity, int64_t num_rows, int64_t dim,
+                             Rows grad, const void* ids, int id_bytes, int64_t n, int64_t padding_idx, float scale,
+                             void* ws, uint64_t ws_bytes, uint64_t* count_host, cudaStream_t st);
 void embedding_check(int device, cudaStream_t st);
 
 void layer_norm(int device, Rows y, float* mean, float* rstd, Rows x, const void* weight, const void* bias,

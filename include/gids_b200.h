@@ -465,7 +465,7 @@ GIDS_API int gids_embedding_check(int device, void *stream);
  * id are zero. Positions whose id is padding_idx (-1: none) or lies outside
  * the table are left out (the latter are reported as above). dweight has the
  * gradient's type or is float32. gids_embedding_grad_workspace: bytes of
- * workspace for this and the two calls below. */
+ * workspace for this and the three calls below. */
 GIDS_API int gids_embedding_grad_workspace(int64_t n, int64_t num_rows, int64_t dim, uint64_t *bytes);
 GIDS_API int gids_embedding_grad(int device, void *dweight, int weight_type, int64_t dweight_stride, int64_t num_rows,
                                  int64_t dim, const void *grad, int grad_type, int64_t grad_stride, const void *ids,
@@ -487,6 +487,16 @@ GIDS_API int gids_embedding_grad_rows(int device, int64_t *rows, void *values, i
                                       int64_t capacity, int64_t num_rows, int64_t dim, const void *grad, int grad_type,
                                       int64_t grad_stride, int64_t n, float scale, void *workspace,
                                       uint64_t workspace_bytes, void *stream);
+
+/* Both in one call, for results that have room for all the rows there can be
+ * (capacity at least min(n, num_rows)): nothing waits between the sort and the
+ * sums. Waits for the stream at the end and returns the number of rows in
+ * count_host (refused with GIDS_E_STATE on a stream that is being captured). */
+GIDS_API int gids_embedding_grad_distinct(int device, int64_t *rows, void *values, int value_type,
+                                          int64_t values_stride, int64_t capacity, int64_t num_rows, int64_t dim,
+                                          const void *grad, int grad_type, int64_t grad_stride, const void *ids,
+                                          int id_bytes, int64_t n, int64_t padding_idx, float scale, void *workspace,
+                                          uint64_t workspace_bytes, uint64_t *count_host, void *stream);
 
 /* y[i, :] = (x[i, :] - m) r * weight + bias with m the mean and r = 1 /
  * sqrt(v + eps), v the mean squared difference from m, of row i. weight and

@@ -145,3 +145,22 @@ def test_modules_build_on_cpu():
     assert n.bias is None and n.weight.shape == (6,)
     assert layers.LayerNorm(6, affine=False).weight is None
     assert "padding_idx=9" in repr(e) and "eps=1e-05" in repr(n)
+
+
+def test_abi_distinct_refusals(built):
+    L = abi()
+    u = ctypes.c_uint64()
+    f = L.gids_embedding_grad_distinct
+    vp, i32, i64, u64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float
+    f.restype = i32
+    f.argtypes = [i32, vp, vp, i32, i64, i64, i64, i64, vp, i32, i64, vp, i32, i64, i64, f32, vp, u64,
+                  ctypes.POINTER(u64), vp]
+    ok = [0, P, P, 0, 8, 4, 10, 8, P, 0, 8, P, 8, 4, -1, 1.0, P, 1 << 30, ctypes.byref(u), None]
+    for i, v in [(0, -1), (1, None), (2, None), (3, 9), (4, 7), (5, 3), (6, -1), (7, 0), (8, None), (9, 9), (10, -1),
+                 (11, None), (12, 3), (13, -1), (14, 10), (16, None), (17, 8), (18, None)]:
+        a = list(ok)
+        a[i] = v
+        assert f(*a) == GIDS_E_INVAL, (i, v)
+    a = list(ok)
+    a[3] = 1
+    assert f(*a) == GIDS_E_UNSUPPORTED

@@ -893,3 +893,37 @@ def test_checking_ids_in_a_capture_is_refused(layers):
     gr.replay()
     torch.cuda.synchronize()
     assert torch.equal(bits(y), bits(layers.layer_norm(g)))
+
+
+def test_distinct_rows_in_one_call_and_in_two(layers, monkeypatch):
+    for n, rows in ((1, 1), (90, 40), (4000, 700), (60000, 3000)):
+        ids, g = randint(rows, (n,), seed=n), randn(n, 40, seed=n, dtype="bf16")
+        got = []
+        for limit in (0, 1 << 40):
+            monkeypatch.setattr(layers, "_ONE_CALL_BYTES", limit)
+            got.append(layers.embedding_grad_rows(ids, g, rows, 0.5, 0, torch.float32))
+        assert all(torch.equal(bits(a), bits(b)) for a, b in zip(*got))
+        assert got[1][0].is_contiguous() and got[1][1].is_contiguous()
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 33, 64, 100, 127, 128])
+def test_distinct_rows_of_few_ids(layers, n):
+    for rows, dim, t in ((5, 16, "f32"), (1 << 31, 8, "bf16"), (300, 1024, "f16")):
+        ids = (randint(1 << 40, (n,), seed=n) * 7919) % rows
+        ids[n // 2:] = ids[: n - n // 2].clone()
+        g = randn(n, dim, seed=n, dtype=t)
+        r, v = layers.embedding_grad_rows(ids, g, rows, 2.0)
+        want, inv = torch.unique(ids, return_inverse=True)
+        s, a, c = group_sums(inv, g, len(want))
+        assert torch.equal(r, want)
+        close(v, 2.0 * s, grad_error(a, c, 2.0, 2.0 * s))
+        # padding and bad ids are left out
+        bad = ids.clone()
+        bad[0] = rows if n > 1 else ids[0]
+        pad = int(ids[-1])
+        r, v = layers.embedding_grad_rows(bad, g, rows, 2.0, pad)
+        if n > 1:
+            with pytest.raises(RuntimeError, match="outside its table"):
+                layers.check_ids(DEV)
+        keep = (bad < rows) & (bad != pad)
+        assert torch.equal(r, torch.unique(bad[keep]))
