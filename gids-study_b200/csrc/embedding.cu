@@ -538,23 +538,6 @@ struct ClusterShared {
   unsigned int heads;
   unsigned long long list[CLUSTER_THREADS * SORT_ITEMS];
 };
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// the address of `p` (of this block's shared memory) in block `rank` of the cluster
-__device__ __forceinline__ unsigned int peer(const void* p, unsigned int rank) {
-  unsigned int r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(r)
-               : "r"((unsigned int)__cvta_generic_to_shared(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ unsigned int peer_load(const unsigned int* p, unsigned int rank) {
-  unsigned int v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer(p, rank)) : "memory");
-  return v;
-}
 
 __global__ void __launch_bounds__(CLUSTER_THREADS) cluster_sort_kernel(IdSource src, unsigned int n, int key_bits,
                                                                        int items, unsigned int blocks,

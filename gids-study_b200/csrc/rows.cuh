@@ -135,6 +135,25 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
+// Blocks of a cluster and their shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// the address of `p` (of this block's shared memory) in block `rank` of the cluster
+__device__ __forceinline__ unsigned int peer(const void* p, unsigned int rank) {
+  unsigned int r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r)
+               : "r"((unsigned int)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ unsigned int peer_load(const unsigned int* p, unsigned int rank) {
+  unsigned int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer(p, rank)) : "memory");
+  return v;
+}
+
 // Two float32 values in one register pair: sm_100a adds, multiplies and fuses
 // both with one instruction, each half rounded as the scalar instruction does.
 struct F2 {

@@ -927,3 +927,15 @@ def test_distinct_rows_of_few_ids(layers, n):
                 layers.check_ids(DEV)
         keep = (bad < rows) & (bad != pad)
         assert torch.equal(r, torch.unique(bad[keep]))
+
+
+@pytest.mark.parametrize("d", [1, 5, 24, 96, 200, 257, 768, 1001, 1024, 4096, 4100, 8192, 9000, 16384])
+def test_norm_gradient_of_few_rows(layers, d):
+    """Around the row counts where one cluster stops doing all of it."""
+    for n in (1, 3, 8, 9, 31, 33, 64, 100, 129, 160, 320, 512, 513, 641, 1300, 2050):
+        if n * d > 3000000:
+            continue
+        for pair in (("bf16", "f32"), ("f32", "f32")):
+            x, w, _ = norm_inputs(n, d, pair, seed=n)
+            _, mean, rstd = layers.layer_norm_stats(x)
+            check_norm_grad(layers, x, w, randn(n, d, seed=2, dtype=pair[0]), mean, rstd)
