@@ -906,11 +906,13 @@ int launch_ln_grad(const LnGradArgs& a, const Layout& l, int sms, cudaStream_t s
   constexpr int U = VEC == 1 ? 16 / (int)sizeof(X) : 1;
   // Few columns a thread (their sums, the parameters and R rows are all in
   // registers) and R rows to a barrier, as long as a block has two groups to
-  // overlap: 262,144 x 1024 bf16 253 us with 4 rows of one vector, 281 us with
-  // 2 rows; 65,536 x 4096 bf16 358 us as one group of 512 threads, 382 us as two of
-  // 256 with 2 rows of two vectors (spills), 280 us with one row.
+  // overlap: 262,144 x 1024 bf16 253 us with 4 rows of one vector, 281 us with 2
+  // rows; 65,536 x 4096 bf16 358 us as one group of 512 threads with 4 rows, 298 us as
+  // two of 256 with one row of two vectors, 272 us with two rows (which spill where the
+  // edges of odd rows take registers too).
   if (group(U) <= LN_THREADS / 2) return launch_ln_grad_k<X, VEC, U, 4>(a, l, sms, st);
-  if (group(2 * U) <= LN_THREADS) return launch_ln_grad_k<X, VEC, 2 * U, 1>(a, l, sms, st);
+  if (group(2 * U) <= LN_THREADS)
+    return l.aligned ? launch_ln_grad_k<X, VEC, 2 * U, 2>(a, l, sms, st) : launch_ln_grad_k<X, VEC, 2 * U, 1>(a, l, sms, st);
   return launch_ln_grad_k<X, VEC, 4 * U, 1>(a, l, sms, st);
 }
 
