@@ -161,13 +161,13 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     m, dev, stream = _store_module(), grad.device, _stream(grad.device)
     n = ids.numel()
     most = min(n, num_rows)
-    if most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
+    if n <= _ONE_CALL_IDS and most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
         rows = grad.new_empty(most, dtype=torch.int64)
         values = grad.new_empty((most, dim), dtype=dtype)
         count = m.embedding_grad_distinct(dev.index, rows.data_ptr(), values.data_ptr(), wt, dim, most, num_rows, dim,
                                           g.data_ptr(), gt, g.stride(0), ids.data_ptr(), ids.element_size(), n, pad,
                                           scale, ws.data_ptr(), ws.numel(), stream)
-        return (rows, values) if count == most else (rows[:count], values[:count])
+        return rows.resize_(count), values.resize_(count, dim)
     count = m.embedding_group(dev.index, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
                               ws.numel(), 0, stream)
     rows = grad.new_empty(count, dtype=torch.int64)
@@ -177,9 +177,11 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     return rows, values
 
 
-# Results up to this size get room for every row there can be, so that one call sorts and
-# sums without a wait between (7,910 ids x 448 bf16: 35 us a pass instead of 44); larger ones
-# wait for the count and hold no more than the rows there are.
+# Up to 128 ids one kernel finds the distinct ids and sums their rows, so one call with room
+# for every row there can be is quicker (8 ids x 128 fp32: 27 us a pass instead of 34); with
+# more ids it is not (7,910 x 448 bf16: 49 us, in two calls 43), and the wait for the count
+# lets the result hold no more than the rows there are. Nor should one call take much room.
+_ONE_CALL_IDS = 128
 _ONE_CALL_BYTES = 8 << 20
 
 

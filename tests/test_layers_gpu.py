@@ -939,3 +939,26 @@ def test_norm_gradient_of_few_rows(layers, d):
             x, w, _ = norm_inputs(n, d, pair, seed=n)
             _, mean, rstd = layers.layer_norm_stats(x)
             check_norm_grad(layers, x, w, randn(n, d, seed=2, dtype=pair[0]), mean, rstd)
+
+
+@pytest.mark.parametrize("n,rows,dim", [(128, 300, 24), (129, 300, 24), (4000, 700, 40), (40000, 3000, 72)])
+def test_distinct_rows_through_the_abi(layers, n, rows, dim):
+    """Rows of the result are strided here, with room for more of them; what lies between and behind stays."""
+    ids, g = randint(rows, (n,), seed=n), randn(n, dim, seed=n, dtype="f16")
+    want_rows, want = layers.embedding_grad_rows(ids, g, rows, 0.5, 7, torch.float32)
+    most, stride = min(n, rows) + 5, dim + 8
+    out_rows = torch.full((most,), -5, dtype=torch.int64, device=DEV)
+    out = torch.full((most, stride), -5.0, device=DEV)
+    ws = torch.empty(layers._store_module().embedding_grad_workspace(n, rows, dim), dtype=torch.uint8, device=DEV)
+    L, count = abi(), ctypes.c_uint64()
+    vp, i32, i64, u64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float
+    L.gids_embedding_grad_distinct.argtypes = [i32, vp, vp, i32, i64, i64, i64, i64, vp, i32, i64, vp, i32, i64, i64,
+                                               f32, vp, u64, ctypes.POINTER(u64), vp]
+    assert L.gids_embedding_grad_distinct(
+        0, out_rows.data_ptr(), out.data_ptr(), 0, stride, most, rows, dim, g.data_ptr(), 1, dim, ids.data_ptr(), 8, n,
+        7, 0.5, ws.data_ptr(), ws.numel(), ctypes.byref(count), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    k = count.value
+    assert k == len(want_rows) and torch.equal(out_rows[:k], want_rows)
+    assert torch.equal(bits(out[:k, :dim]), bits(want))
+    assert bool((out_rows[k:] == -5).all()) and bool((out[k:] == -5).all()) and bool((out[:, dim:] == -5).all())
