@@ -476,7 +476,8 @@ class GIDS:
             current_access += n_access(batch)
             num_iter += 1
             required_accesses += self.prev_cpu_access
-            if current_access > required_accesses:
+            # no number of batches without a stored row would reach it
+            if current_access > required_accesses or (self.node_embeddings and n_access(batch) == 0):
                 break
 
         outs, idxs, ns, keys = [], [], [], []

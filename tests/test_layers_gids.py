@@ -102,3 +102,14 @@ def test_constructor_refusals(fake):  # noqa: F811
         fake(node_embeddings={"author": Table(3, 4)})
     with pytest.raises(ValueError, match="heterograph"):
         fake(feature_norm={"author": Table(3, 4)})
+
+
+def test_accumulator_with_nothing_stored_takes_one_batch_at_a_time(fake):  # noqa: F811
+    t = Table(100, 4)
+    g = fake(heterograph=True, heterograph_map=MAP, node_embeddings={"author": t}, accumulator_flag=True)
+    bs = hetero(5, seed=3, sizes={"author": 7})
+    it = iter([list(b) for b in bs])
+    for i, b in enumerate(bs):
+        out = g.fetch_feature(64, it, "cpu")
+        assert out[1] == b[1] and torch.equal(out[-1]["author"], t.rows[b[0]["author"]])
+    assert len(t.seen) == 5
