@@ -1370,6 +1370,7 @@ std::mutex g_words_mu;
 std::vector<unsigned long long*> g_words;
 struct HostWord {
   unsigned long long *host = nullptr, *dev = nullptr;
+  bool done = false;  // no kernel is left that writes it
   explicit HostWord(bool wanted) {
     if (!wanted) return;
     {
@@ -1385,10 +1386,11 @@ struct HostWord {
   }
   unsigned long long wait(cudaStream_t st) {
     GIDS_CUDA(cudaStreamSynchronize(st));
+    done = true;
     return *reinterpret_cast<volatile unsigned long long*>(host);
   }
   ~HostWord() {
-    if (!host) return;
+    if (!done) return;  // a call that failed half way: another one must not get this word
     std::lock_guard<std::mutex> lk(g_words_mu);
     g_words.push_back(host);
   }
