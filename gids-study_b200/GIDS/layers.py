@@ -130,9 +130,15 @@ def _grad_args(ids, grad, num_rows, dtype):
     dtype = grad.dtype if dtype is None else dtype
     gt, wt = _type(grad.dtype, "grad"), _type(dtype, "dtype")
     _need_cuda(grad.device, ids)
-    rows = _as_rows(grad, dim)
-    ws = grad.new_empty(_store_module().embedding_grad_workspace(ids.numel(), num_rows, dim), dtype=torch.uint8)
-    return ids, rows, dim, dtype, gt, wt, ws
+    return ids, _as_rows(grad, dim), dim, dtype, gt, wt
+
+
+def _grad_workspace(grad, n, num_rows, dim):
+    return grad.new_empty(_store_module().embedding_grad_workspace(n, num_rows, dim), dtype=torch.uint8)
+
+
+_FEW_IDS = 128  # GIDS_FEW_IDS: up to here one kernel, without a workspace
+_FEW_NORM = 1 << 18  # GIDS_FEW_NORM
 
 
 def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None):
@@ -142,11 +148,13 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None)
     Ids equal to ``padding_idx`` are left out."""
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
-    ids, g, dim, dtype, gt, wt, ws = _grad_args(ids, grad, num_rows, dtype)
+    ids, g, dim, dtype, gt, wt = _grad_args(ids, grad, num_rows, dtype)
+    n = ids.numel()
+    ws = None if n <= _FEW_IDS else _grad_workspace(grad, n, num_rows, dim)
     dw = grad.new_empty((num_rows, dim), dtype=dtype)
     _store_module().embedding_grad(grad.device.index, dw.data_ptr(), wt, dim, num_rows, dim, g.data_ptr(), gt,
-                                   g.stride(0), ids.data_ptr(), ids.element_size(), ids.numel(), pad, scale,
-                                   ws.data_ptr(), ws.numel(), _stream(grad.device))
+                                   g.stride(0), ids.data_ptr(), ids.element_size(), n, pad, scale,
+                                   *_span(ws), _stream(grad.device))
     return dw
 
 
@@ -157,17 +165,18 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     number of rows, so it cannot be captured into a graph."""
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
-    ids, g, dim, dtype, gt, wt, ws = _grad_args(ids, grad, num_rows, dtype)
+    ids, g, dim, dtype, gt, wt = _grad_args(ids, grad, num_rows, dtype)
     m, dev, stream = _store_module(), grad.device, _stream(grad.device)
     n = ids.numel()
     most = min(n, num_rows)
-    if n <= _ONE_CALL_IDS and most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
+    if n <= _FEW_IDS and most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
         rows = grad.new_empty(most, dtype=torch.int64)
         values = grad.new_empty((most, dim), dtype=dtype)
         count = m.embedding_grad_distinct(dev.index, rows.data_ptr(), values.data_ptr(), wt, dim, most, num_rows, dim,
                                           g.data_ptr(), gt, g.stride(0), ids.data_ptr(), ids.element_size(), n, pad,
-                                          scale, ws.data_ptr(), ws.numel(), stream)
+                                          scale, 0, 0, stream)
         return rows.resize_(count), values.resize_(count, dim)
+    ws = _grad_workspace(grad, n, num_rows, dim)
     count = m.embedding_group(dev.index, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
                               ws.numel(), 0, stream)
     rows = grad.new_empty(count, dtype=torch.int64)
@@ -177,11 +186,10 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     return rows, values
 
 
-# Up to 128 ids one kernel finds the distinct ids and sums their rows, so one call with room
+# Up to _FEW_IDS ids one kernel finds the distinct ids and sums their rows, so one call with room
 # for every row there can be is quicker (8 ids x 128 fp32: 27 us a pass instead of 34); with
 # more ids it is not (7,910 x 448 bf16: 49 us, in two calls 43), and the wait for the count
 # lets the result hold no more than the rows there are. Nor should one call take much room.
-_ONE_CALL_IDS = 128
 _ONE_CALL_BYTES = 8 << 20
 
 
@@ -281,6 +289,11 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _span(ws):
+    """Address and bytes of a workspace, or none."""
+    return (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
+
+
 def _layer_norm_forward(x, weight, bias, eps, stats):
     dim, xt, pt = _params(x, weight, bias)
     _need_cuda(x.device, weight, bias)
@@ -317,14 +330,14 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
         if s.dtype != torch.float32 or s.numel() != n or not s.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 tensor of {n} elements")
     m = _store_module()
-    want_p = need[1] or need[2]
+    few = dim <= 4096 and n * max(dim, 128) <= _FEW_NORM  # no workspace
     dx = _new_like(x) if need[0] else None
     dw = x.new_empty(dim, dtype=ptype) if need[1] else None
     db = x.new_empty(dim, dtype=ptype) if need[2] else None
-    ws = x.new_empty(m.layer_norm_grad_workspace(n, dim) if want_p else 0, dtype=torch.uint8)
+    ws = None if few or not (need[1] or need[2]) else x.new_empty(m.layer_norm_grad_workspace(n, dim), dtype=torch.uint8)
     m.layer_norm_grad(x.device.index, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
                       gr.stride(0), xr.data_ptr(), xt, xr.stride(0), _ptr(weight), pt, mean.data_ptr(),
-                      rstd.data_ptr(), n, dim, ws.data_ptr(), ws.numel(), _stream(x.device))
+                      rstd.data_ptr(), n, dim, *_span(ws), _stream(x.device))
     return dx, dw, db
 
 

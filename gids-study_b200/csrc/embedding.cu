@@ -929,11 +929,11 @@ __global__ void __launch_bounds__(SEG_THREADS) join_kernel(SegArgs a) {
 // The gradient of a few ids in one kernel: every warp looks for its ids in the
 // whole list instead of in a sorted one. A warp takes an id's first position and
 // a slab of columns and adds the rows of the positions that share the id. Dense:
-// it also zeroes table rows that no id names. Distinct rows (rows_out): an id's
+// it also zeroes table rows that no id names. Distinct rows: an id's
 // row is the number of smaller ids. The additions are those of
 // segment_kernel and join_kernel, chunk by chunk and block by block of the
 // sorted list, so that the dense form and the distinct rows hold the same bits.
-constexpr unsigned int TINY_IDS = 128;
+constexpr unsigned int TINY_IDS = GIDS_FEW_IDS;
 constexpr int TINY_THREADS = 256;
 
 struct TinyArgs {
@@ -944,14 +944,16 @@ struct TinyArgs {
   unsigned int n, slabs;
   unsigned int chunk, rows;  // words of a chunk and of a block (powers of two)
   float scale;
-  long long* rows_out;  // null: dense
+  unsigned int zero_rows;  // dense: rows that a warp zeroes at a time
+  bool distinct;
   unsigned int capacity;
-  volatile unsigned long long* host_count;  // with rows_out: how many
+  long long* rows_out;                      // of the distinct rows
+  volatile unsigned long long* host_count;  // how many there are
 };
 
 template <typename G, typename W, int VEC>
 __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
-  constexpr int P = VEC / 2, WORDS = TINY_IDS / 32;
+  constexpr int P = (VEC + 1) / 2, WORDS = TINY_IDS / 32;
   __shared__ unsigned int keys[TINY_IDS];
   const unsigned int none = (unsigned int)a.src.num_rows;  // padding, bad ids and the list's end
   for (unsigned int i = threadIdx.x; i < TINY_IDS; i += TINY_THREADS)
@@ -966,10 +968,10 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
   for (int w = 0; w < WORDS; w++) {
     mine[w] = keys[w * 32 + lane];
     lead[w] = mine[w] != none;
-    if (a.rows_out)
+    if (a.distinct)
       for (unsigned int j = 0; j < w * 32 + lane; j++) lead[w] = lead[w] && keys[j] != mine[w];
   }
-  if (a.rows_out && blockIdx.x == 0 && threadIdx.x < 32) {
+  if (a.distinct && blockIdx.x == 0 && threadIdx.x < 32) {
     unsigned int all = 0;
 #pragma unroll
     for (int w = 0; w < WORDS; w++) all += __popc(__ballot_sync(0xffffffffu, lead[w]));
@@ -986,16 +988,16 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
     unsigned int at[WORDS];
     lookup(key, at);
     // index: where the id's run starts in the sorted list; row: of the result
-    unsigned int first = TINY_IDS, left = 0, index = 0, row = a.rows_out ? 0 : key;
+    unsigned int first = TINY_IDS, left = 0, index = 0, row = a.distinct ? 0 : key;
 #pragma unroll
     for (int w = WORDS - 1; w >= 0; w--) {
       if (at[w]) first = w * 32 + __ffs(at[w]) - 1;
       left += __popc(at[w]);
       index += __popc(__ballot_sync(0xffffffffu, mine[w] < key));
-      if (a.rows_out) row += __popc(__ballot_sync(0xffffffffu, lead[w] && mine[w] < key));
+      if (a.distinct) row += __popc(__ballot_sync(0xffffffffu, lead[w] && mine[w] < key));
     }
     if (key == none || first != i || col >= a.dim || row >= a.capacity) continue;  // (no shuffles below)
-    if (a.rows_out && col == 0) a.rows_out[row] = (long long)key;
+    if (a.distinct && col == 0) a.rows_out[row] = (long long)key;
     // sums of the chunk, of the block up to the chunk, of the run up to the block
     F2 acc[P], blk[P], tot[P];
     bool in_blk = false, in_tot = false;
@@ -1054,7 +1056,12 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
         }
         index++;
 #pragma unroll
-        for (int p = 0; p < P; p++) acc[p] = add2(acc[p], pair_of(v[u], p));
+        for (int p = 0; p < P; p++) {
+          if constexpr (VEC == 1)
+            acc[p] = add2(acc[p], F2(to_f32(v[u][0].v[0]), 0.0f));
+          else
+            acc[p] = add2(acc[p], pair_of(v[u], p));
+        }
       }
       left -= some;
     }
@@ -1067,17 +1074,39 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
     for (int j = 0; j < VEC; j++) f[j] = a.scale * (j & 1 ? acc[j / 2].hi() : acc[j / 2].lo());
     store_vec<W, VEC>(reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride + col, f);
   }
-  if (a.rows_out) return;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  const long long pieces = a.dim * (long long)sizeof(W) / 16;  // (whole: rows are in vectors)
-  for (unsigned long long row = warp; row < none; row += warps) {  // (none may be close to 2^32)
-    unsigned int at[WORDS], any = 0;
-    lookup((unsigned int)row, at);
+  if (a.distinct) return;
+  W* table = reinterpret_cast<W*>(a.out);
+  const auto clear_span = [&](W* out, long long left) {
+    if constexpr (VEC == 1) {  // the elements before the first boundary of 16 bytes
+      const int head = (int)min((long long)((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / (int)sizeof(W), left);
+      if ((int)lane < head) out[lane] = from_f32<W>(0.0f);
+      out += head;
+      left -= head;
+    }
+    constexpr int PER = 16 / (int)sizeof(W);
+    const long long pieces = left / PER;
+    for (long long c = lane; c < pieces; c += 32) reinterpret_cast<uint4*>(out)[c] = make_uint4(0, 0, 0, 0);
+    if (VEC == 1 && (int)lane < (int)(left - pieces * PER)) out[pieces * PER + lane] = from_f32<W>(0.0f);
+  };
+  // zero_rows rows at a time, of which few hold a row of the gradient
+  const unsigned long long step = (unsigned long long)warps * a.zero_rows;
+  for (unsigned long long base = (unsigned long long)warp * a.zero_rows; base < none; base += step) {
+    const unsigned int count = (unsigned int)min((unsigned long long)a.zero_rows, none - base);
+    bool hit = false;
 #pragma unroll
-    for (int w = 0; w < WORDS; w++) any |= at[w];
-    if (any) continue;
-    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<W*>(a.out) + (long long)row * a.out_stride);
-    for (long long c = lane; c < pieces; c += 32) out[c] = zero;
+    for (int w = 0; w < WORDS; w++) hit = hit || mine[w] - (unsigned int)base < count;  // (`none` lies behind)
+    const bool some = __any_sync(0xffffffffu, hit);
+    if (!some && a.out_stride == a.dim) {
+      clear_span(table + (long long)base * a.dim, (long long)count * a.dim);
+      continue;
+    }
+    for (unsigned int r = 0; r < count; r++) {
+      unsigned int at[WORDS], any = 0;
+      lookup((unsigned int)base + r, at);
+#pragma unroll
+      for (int w = 0; w < WORDS; w++) any |= at[w];
+      if (!any) clear_span(table + (long long)(base + r) * a.out_stride, a.dim);
+    }
   }
 }
 
@@ -1299,34 +1328,37 @@ void segments(const SegArgs& a, const Rows& out, const Rows& grad, bool first, c
   return launch_segments_vec<__nv_bfloat16, __nv_bfloat16>(a, out, grad, first, st);
 }
 
-// Whether a gradient goes to tiny_grad_kernel: few ids, rows in vectors. (64 ids
-// into 5,000 x 128 fp32, dense: 16 us a pass by the sorted list, 12 this way.)
-bool tiny_grad(int64_t n, int64_t dim, const Rows& out, const Rows& grad) {
-  const int vec = 16 / type_bytes(grad.type);
-  return n <= (int64_t)TINY_IDS && vec_ok(out, dim, vec) && vec_ok(grad, dim, vec);
-}
-
-template <typename G, typename W>
+template <typename G, typename W, int VEC>
 void launch_tiny(TinyArgs a, int sms, cudaStream_t st) {
-  constexpr int VEC = 16 / (int)sizeof(G);
   a.slabs = (unsigned int)((a.dim + 32 * VEC - 1) / (32 * VEC));
   const SegPlan plan = seg_plan(a.n, (uint64_t)a.dim, sizeof(G));
   a.chunk = plan.chunk;
   a.rows = plan.rows;
-  const uint64_t tasks = std::max<uint64_t>((uint64_t)a.n * a.slabs, a.rows_out ? 0 : a.src.num_rows);
+  // about 2 KB of zeros at a time
+  a.zero_rows = (unsigned int)std::clamp<int64_t>(2048 / (a.dim * (int64_t)sizeof(W)), 1, 32);
+  const uint64_t tasks =
+      std::max<uint64_t>((uint64_t)a.n * a.slabs, a.distinct ? 0 : (a.src.num_rows + a.zero_rows - 1) / a.zero_rows);
   const unsigned int grid = (unsigned int)std::min<uint64_t>((tasks + 7) / 8, (uint64_t)sms * 8);
   tiny_grad_kernel<G, W, VEC><<<grid, TINY_THREADS, 0, st>>>(a);
   GIDS_CUDA(cudaGetLastError());
 }
 
+template <typename G, typename W>
+void launch_tiny_vec(const TinyArgs& a, const Rows& out, const Rows& grad, int sms, cudaStream_t st) {
+  constexpr int BIG = 16 / (int)sizeof(G);
+  if (vec_ok(out, a.dim, BIG) && vec_ok(grad, a.dim, BIG)) return launch_tiny<G, W, BIG>(a, sms, st);
+  launch_tiny<G, W, 1>(a, sms, st);
+}
+
+// (64 ids into 5,000 x 128 fp32, dense: 16 us a pass by the sorted list, 12 this way.)
 void tiny(const TinyArgs& a, const Rows& out, const Rows& grad, int sms, cudaStream_t st) {
   if (out.type == GIDS_F32) {
-    if (grad.type == GIDS_F32) return launch_tiny<float, float>(a, sms, st);
-    if (grad.type == GIDS_F16) return launch_tiny<__half, float>(a, sms, st);
-    return launch_tiny<__nv_bfloat16, float>(a, sms, st);
+    if (grad.type == GIDS_F32) return launch_tiny_vec<float, float>(a, out, grad, sms, st);
+    if (grad.type == GIDS_F16) return launch_tiny_vec<__half, float>(a, out, grad, sms, st);
+    return launch_tiny_vec<__nv_bfloat16, float>(a, out, grad, sms, st);
   }
-  if (out.type == GIDS_F16) return launch_tiny<__half, __half>(a, sms, st);
-  launch_tiny<__nv_bfloat16, __nv_bfloat16>(a, sms, st);
+  if (out.type == GIDS_F16) return launch_tiny_vec<__half, __half>(a, out, grad, sms, st);
+  launch_tiny_vec<__nv_bfloat16, __nv_bfloat16>(a, out, grad, sms, st);
 }
 
 template <typename W, typename O, int VEC>
@@ -1406,7 +1438,9 @@ IdSource id_source(const void* ids, int id_bytes, int64_t num_rows, int64_t padd
   return s;
 }
 
-void check_workspace(const void* ws, uint64_t ws_bytes, const Workspace& lay) {
+// few: the call's kernel needs none, so there may be none (null, 0 bytes)
+void check_workspace(const void* ws, uint64_t ws_bytes, const Workspace& lay, bool few = false) {
+  if (few && !ws && !ws_bytes) return;
   GIDS_CHECK(ws && ((uintptr_t)ws) % 256 == 0, GIDS_E_INVAL, "workspace is null or not aligned to 256 bytes");
   GIDS_CHECK(ws_bytes >= lay.bytes, GIDS_E_INVAL,
              "workspace too small: " + std::to_string(lay.bytes) + " bytes are needed");
@@ -1499,11 +1533,11 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
   GIDS_CHECK(padding_idx >= -1 && padding_idx < std::max<int64_t>(num_rows, 1), GIDS_E_INVAL,
              "padding_idx must be -1 (none) or a row");
   const Workspace lay((uint64_t)n, (uint64_t)dim);
-  if (n) check_workspace(ws, ws_bytes, lay);
+  if (n) check_workspace(ws, ws_bytes, lay, n <= (int64_t)TINY_IDS);
   check_id_errors(device);
   if (num_rows == 0 && n == 0) return;
   DeviceGuard dg(device);
-  if (n > 0 && tiny_grad(n, dim, dweight, grad)) {
+  if (n > 0 && n <= (int64_t)TINY_IDS) {
     TinyArgs t{};
     t.src = id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device));
     t.out = dweight.p;
@@ -1550,12 +1584,12 @@ void embedding_grad(int device, Rows dweight, int64_t num_rows, int64_t dim, Row
 namespace {
 // Checks of the calls that return the number of distinct rows to the host.
 void check_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
-                 int64_t dim, const void* ws, uint64_t ws_bytes) {
+                 int64_t dim, const void* ws, uint64_t ws_bytes, bool few) {
   check_device(device);
   check_ids(ids, id_bytes, n, num_rows, dim);
   GIDS_CHECK(padding_idx >= -1 && padding_idx < std::max<int64_t>(num_rows, 1), GIDS_E_INVAL,
              "padding_idx must be -1 (none) or a row");
-  check_workspace(ws, ws_bytes, Workspace((uint64_t)n, (uint64_t)dim));
+  check_workspace(ws, ws_bytes, Workspace((uint64_t)n, (uint64_t)dim), few);
 }
 void check_not_capturing(cudaStream_t st) {
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -1598,7 +1632,7 @@ void sum_rows(int64_t* rows, const Rows& values, int64_t capacity, int64_t num_r
 void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx,
                      int64_t dim, void* ws, uint64_t ws_bytes, uint64_t* count_dev, uint64_t* count_host,
                      cudaStream_t st) {
-  check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes);
+  check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes, false);
   check_id_errors(device);
   DeviceGuard dg(device);
   if (count_host) check_not_capturing(st);
@@ -1632,7 +1666,7 @@ void embedding_grad_rows(int device, int64_t* rows, Rows values, int64_t capacit
 void embedding_grad_distinct(int device, int64_t* rows, Rows values, int64_t capacity, int64_t num_rows, int64_t dim,
                              Rows grad, const void* ids, int id_bytes, int64_t n, int64_t padding_idx, float scale,
                              void* ws, uint64_t ws_bytes, uint64_t* count_host, cudaStream_t st) {
-  check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes);
+  check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes, n <= (int64_t)TINY_IDS);
   check_values(rows, values, capacity, grad, n, dim);
   GIDS_CHECK(capacity >= std::min(n, num_rows), GIDS_E_INVAL, "capacity must be at least min(n, num_rows)");
   check_id_errors(device);
@@ -1640,10 +1674,8 @@ void embedding_grad_distinct(int device, int64_t* rows, Rows values, int64_t cap
   check_not_capturing(st);
   *count_host = 0;
   if (n == 0) return;
-  const Workspace lay((uint64_t)n, (uint64_t)dim);
-  char* base = static_cast<char*>(ws);
   HostWord word(true);
-  if (tiny_grad(n, dim, values, grad) && capacity) {
+  if (n <= (int64_t)TINY_IDS) {
     TinyArgs t{};
     t.src = id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device));
     t.out = values.p;
@@ -1653,6 +1685,7 @@ void embedding_grad_distinct(int device, int64_t* rows, Rows values, int64_t cap
     t.dim = dim;
     t.n = (unsigned int)n;
     t.scale = scale;
+    t.distinct = true;
     t.rows_out = reinterpret_cast<long long*>(rows);
     t.capacity = (unsigned int)std::min<int64_t>(capacity, n);
     t.host_count = word.dev;
@@ -1660,6 +1693,8 @@ void embedding_grad_distinct(int device, int64_t* rows, Rows values, int64_t cap
     *count_host = word.wait(st);
     return;
   }
+  const Workspace lay((uint64_t)n, (uint64_t)dim);
+  char* base = static_cast<char*>(ws);
   sort_ids(id_source(ids, id_bytes, num_rows, padding_idx, id_error_word(device)), (uint64_t)n, base, lay, ZeroFill{},
            true, reinterpret_cast<unsigned long long*>(base + lay.count), word.dev, 1, st);
   if (capacity) sum_rows(rows, values, capacity, num_rows, dim, grad, n, scale, base, lay, false, st);

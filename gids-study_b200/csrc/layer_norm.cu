@@ -853,8 +853,10 @@ void launch_ln(const LnArgs& a, const Layout& l, int sms, cudaStream_t st) {
 }
 
 // Few rows go to one cluster, which also adds up dw and db: a launch less (129 x
-// 768 fp16: 18.7 us a pass by two kernels, 17.2 this way).
+// 768 fp16: 18.7 us a pass by two kernels, 17.2 this way). Those that `few` names need
+// no workspace for certain; others go there where a group has up to CLUSTER_STEPS steps.
 constexpr int CLUSTER = 8, CLUSTER_STEPS = 4;
+bool few(int64_t n, int64_t dim) { return dim <= 4096 && n <= GIDS_FEW_NORM / std::max<int64_t>(dim, 128); }
 
 // Returns the partial rows left in a.part.
 template <typename X, int VEC, int K, int R, int GROUP = 0>
@@ -862,7 +864,8 @@ int launch_ln_grad_k(LnGradArgs a, const Layout& l, int sms, cudaStream_t st) {
   constexpr int STAGES = stages_of(2 * VEC * (int)sizeof(X) * K * R);
   Plan p = plan_of<VEC>(a.n, a.dim, K, R, LN_THREADS, l, sms, max_parts(sms));
   const int most = std::min(LN_THREADS / p.group, p.group > 32 ? 15 : LN_THREADS);
-  const bool small = a.part && a.n <= (int64_t)CLUSTER_STEPS * CLUSTER * most * R;
+  const bool small =
+      (a.dw || a.db) && (few(a.n, a.dim) || a.n <= (int64_t)CLUSTER_STEPS * CLUSTER * most * R);
   if (small) {
     a.part = nullptr;
     p.groups = most;
@@ -1040,7 +1043,7 @@ void layer_norm_grad(int device, Rows dx, void* dweight, void* dbias, Rows grad,
   check_param(mean, GIDS_F32, "mean");
   check_param(rstd, GIDS_F32, "rstd");
   const bool params = dweight || dbias;
-  if (params && n) {
+  if (params && n && !(few(n, dim) && !ws && !ws_bytes)) {
     GIDS_CHECK(ws && ((uintptr_t)ws) % 256 == 0, GIDS_E_INVAL, "workspace is null or not aligned to 256 bytes");
     GIDS_CHECK(ws_bytes >= layer_norm_grad_workspace(n, dim), GIDS_E_INVAL,
                "workspace too small: " + std::to_string(layer_norm_grad_workspace(n, dim)) + " bytes are needed");

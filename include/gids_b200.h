@@ -448,6 +448,13 @@ GIDS_API int gids_out_degree(int device, const void *indices, int index_bytes, u
 #define GIDS_F16 1
 #define GIDS_BF16 2
 
+/* Small calls that need no workspace: gids_embedding_grad and
+ * gids_embedding_grad_distinct of up to GIDS_FEW_IDS ids, and
+ * gids_layer_norm_grad with dim <= 4096 and n * max(dim, 128) <=
+ * GIDS_FEW_NORM. They may be given none (NULL, 0 bytes). */
+#define GIDS_FEW_IDS 128
+#define GIDS_FEW_NORM (1 << 18)
+
 /* out[i, :] = scale * weight[ids[i], :], i < n, `dim` columns of a table of
  * num_rows rows. ids: int32 or int64 (id_bytes 4 or 8). out has the table's
  * type, or any type if the table is float32; in the table's type a scale of 1
@@ -490,7 +497,7 @@ GIDS_API int gids_embedding_grad_rows(int device, int64_t *rows, void *values, i
 
 /* Both in one call, for results that have room for all the rows there can be
  * (capacity at least min(n, num_rows)): nothing waits between the sort and the
- * sums, and up to 128 ids take one kernel. Waits for the stream at the end and
+ * sums, and up to GIDS_FEW_IDS ids take one kernel. Waits for the stream at the end and
  * returns the number of rows in count_host (refused with GIDS_E_STATE on a stream
  * that is being captured). */
 GIDS_API int gids_embedding_grad_distinct(int device, int64_t *rows, void *values, int value_type,

@@ -164,3 +164,36 @@ def test_abi_distinct_refusals(built):
     a = list(ok)
     a[3] = 1
     assert f(*a) == GIDS_E_UNSUPPORTED
+
+
+def test_abi_small_calls_may_go_without_a_workspace(built):
+    """NULL with 0 bytes is refused where a workspace is needed, and not before the other arguments are
+    looked at where none is; NULL with a size is an error everywhere."""
+    L = abi()
+    none = dict(ws=None, wsb=0)
+    assert grad(L, n=129, **none) == GIDS_E_INVAL
+    assert grad(L, n=128, ws=None, wsb=256) == GIDS_E_INVAL
+    for n, d in ((2049, 128), (2049, 1), (65, 4096), (1, 4097), (1 << 37, 8)):
+        assert norm_grad(L, n=n, dim=d, dxs=d, gs=d, xs=d, **none) == GIDS_E_INVAL, (n, d)
+    assert norm_grad(L, n=4, dim=8, ws=None, wsb=8) == GIDS_E_INVAL
+    u = ctypes.c_uint64()
+    a = [0, P, 8, 4, 10, -1, 8, None, 0, P, None, None]
+    assert L.gids_embedding_group(*a) == GIDS_E_INVAL
+    b = [0, P, P, 0, 8, 3, 10, 8, P, 0, 8, 4, 1.0, None, 0, None]
+    assert L.gids_embedding_grad_rows(*b) == GIDS_E_INVAL
+    vp, i32, i64, u64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float
+    f = L.gids_embedding_grad_distinct
+    f.argtypes = [i32, vp, vp, i32, i64, i64, i64, i64, vp, i32, i64, vp, i32, i64, i64, f32, vp, u64,
+                  ctypes.POINTER(u64), vp]
+    assert f(0, P, P, 0, 8, 10, 10, 8, P, 0, 8, P, 8, 129, -1, 1.0, None, 0, ctypes.byref(u), None) == GIDS_E_INVAL
+
+
+def test_few_constants_match_the_header(built):
+    import pathlib
+    import re
+
+    from GIDS import layers
+
+    text = (pathlib.Path(gids_abi.__file__).parents[1] / "include" / "gids_b200.h").read_text()
+    assert int(re.search(r"#define GIDS_FEW_IDS (\d+)", text)[1]) == layers._FEW_IDS
+    assert eval(re.search(r"#define GIDS_FEW_NORM (.+)", text)[1]) == layers._FEW_NORM

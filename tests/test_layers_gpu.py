@@ -962,3 +962,47 @@ def test_distinct_rows_through_the_abi(layers, n, rows, dim):
     assert k == len(want_rows) and torch.equal(out_rows[:k], want_rows)
     assert torch.equal(bits(out[:k, :dim]), bits(want))
     assert bool((out_rows[k:] == -5).all()) and bool((out[k:] == -5).all()) and bool((out[:, dim:] == -5).all())
+
+
+@pytest.mark.parametrize("dim", [1, 3, 4, 7, 8, 33, 129, 1001])
+def test_few_ids_and_rows_of_any_width(layers, dim):
+    """Up to 128 ids, tables dense and as distinct rows: whole blocks of zero rows, blocks with
+    some, rows on and off 16 bytes."""
+    for n, rows in ((1, 1), (3, 31), (64, 33), (128, 1000), (128, 20000), (5, 70001)):
+        for pair in (("f32", "f32"), ("bf16", "f32"), ("f16", "f16")):
+            g = randn(n, dim, seed=n, dtype=pair[0])
+            check_grad(layers, randint(rows, (n,), seed=rows), g, rows, 0.5, rows // 2, TYPES[pair[1]])
+    # the same bits as the sums of a sorted list that ends in padding
+    ids, g = randint(40, (128,), seed=3), randn(128, dim, seed=3)
+    more = torch.cat([ids + 1, torch.zeros(72, dtype=ids.dtype, device=DEV)])
+    dw = layers.embedding_grad(ids + 1, g, 41, 2.0, 0)
+    assert not bool(dw[0].any())
+    s, a, c = group_sums(more, torch.cat([g, randn(72, dim)]), 41, 0)
+    close(layers.embedding_grad(more, torch.cat([g, randn(72, dim)]), 41, 2.0, 0), 2.0 * s, grad_error(a, c, 2.0, 2.0 * s))
+    close(dw, 2.0 * s, grad_error(a, c, 2.0, 2.0 * s))
+
+
+def test_few_ids_into_a_gapped_table(layers):
+    L = abi()
+    for dim, stride, t, code in ((8, 12, torch.float32, 0), (5, 7, torch.float16, 1), (8, 24, torch.bfloat16, 2)):
+        ids, g = randint(500, (90,), seed=dim), randn(90, dim).to(t)
+        dw = torch.full((502, stride), 7.0, device=DEV, dtype=t)
+        check(L.gids_embedding_grad(0, dw[1:].data_ptr(), code, stride, 500, dim, g.data_ptr(), code, dim,
+                                    ids.data_ptr(), 8, 90, 3, 1.0, None, 0, None))
+        torch.cuda.synchronize()
+        assert torch.equal(bits(dw[1:-1, :dim].contiguous()), bits(layers.embedding_grad(ids, g, 500, 1.0, 3)))
+        assert bool((dw[0] == 7).all()) and bool((dw[-1] == 7).all()) and bool((dw[1:-1, dim:] == 7).all())
+
+
+@pytest.mark.parametrize("n,d", [(2048, 1), (2048, 128), (1000, 8), (341, 768), (63, 4096), (64, 4096), (261, 1001),
+                                 (2000, 130)])
+def test_norm_gradient_without_a_workspace(layers, n, d):
+    """As large as it may be, also where the matrices do not meet 16 bytes alike."""
+    for pair in (("bf16", "f32"), ("f32", "f32"), ("f16", "f16")):
+        x, w, _ = norm_inputs(n, d, pair, seed=n)
+        g = randn(n, d, seed=2, dtype=pair[0])
+        _, mean, rstd = layers.layer_norm_stats(x)
+        check_norm_grad(layers, x, w, g, mean, rstd)
+        wide = torch.zeros(n, d + 3, dtype=x.dtype, device=DEV)
+        wide[:, 1:d + 1] = x
+        check_norm_grad(layers, wide[:, 1:d + 1], w, g, mean, rstd)
