@@ -52,16 +52,15 @@ def _type(t: torch.dtype, what: str) -> int:
     return _TYPES[t]
 
 
-def _need_cuda(device: torch.device, *tensors):
-    if device.type != "cuda":
-        raise ValueError(f"CUDA tensors expected, not {device}")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"a tensor is on {t.device}, the others on {device}")
-
-
-def _stream(device: torch.device) -> int:
-    return _raw_stream(device.index)
+def _device_of(first: torch.Tensor, *others) -> int:
+    """Index of the CUDA device that the tensors (or None) are all on."""
+    device = first.get_device()
+    if device < 0:
+        raise ValueError(f"CUDA tensors expected, not {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor is on {t.device}, the others on {first.device}")
+    return device
 
 
 def _check_ids(ids: torch.Tensor) -> torch.Tensor:
@@ -72,7 +71,10 @@ def _check_ids(ids: torch.Tensor) -> torch.Tensor:
 
 def _as_rows(t: torch.Tensor, dim: int) -> torch.Tensor:
     """t as a matrix of rows [*, dim] whose columns are consecutive (a view where there is one)."""
-    if t.dim() != 2:
+    if t.dim() == 2:
+        if t.is_contiguous():
+            return t
+    else:
         t = t.reshape(-1, dim)
     if (dim > 1 and t.stride(1) != 1) or t.stride(0) < 0:
         t = t.contiguous()
@@ -99,7 +101,7 @@ def check_ids(device=None):
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
-    _store_module().embedding_check(device.index, _stream(device))
+    _store_module().embedding_check(device.index, _raw_stream(device.index))
 
 
 # ------------------------------------------------------------------ embedding
@@ -108,15 +110,16 @@ def _embedding_forward(ids, weight, scale, dtype):
         raise ValueError(f"weight must be a matrix, not {tuple(weight.shape)}")
     num_rows, dim = weight.shape
     wt, ot = _type(weight.dtype, "weight"), _type(dtype, "dtype")
-    _need_cuda(weight.device, ids)
+    device = _device_of(weight, ids)
     if dim > 1 and weight.stride(1) != 1:
         raise ValueError("the columns of weight must be consecutive (stride 1)")
     ids = _check_ids(ids)
-    out = weight.new_empty((*ids.shape, dim), dtype=dtype)
+    shape = (*ids.shape, dim)
+    out = weight.new_empty(shape) if ot == wt else weight.new_empty(shape, dtype=dtype)
     if dim:
-        _store_module().embedding(weight.device.index, out.data_ptr(), ot, dim, weight.data_ptr(), wt,
+        _store_module().embedding(device, out.data_ptr(), ot, dim, weight.data_ptr(), wt,
                                   weight.stride(0), num_rows, dim, ids.data_ptr(), ids.element_size(), ids.numel(),
-                                  scale, _stream(weight.device))
+                                  scale, _raw_stream(device))
     return out
 
 
@@ -129,8 +132,7 @@ def _grad_args(ids, grad, num_rows, dtype):
         raise ValueError("grad has no columns")
     dtype = grad.dtype if dtype is None else dtype
     gt, wt = _type(grad.dtype, "grad"), _type(dtype, "dtype")
-    _need_cuda(grad.device, ids)
-    return ids, _as_rows(grad, dim), dim, dtype, gt, wt
+    return ids, _as_rows(grad, dim), dim, dtype, gt, wt, _device_of(grad, ids)
 
 
 def _grad_workspace(grad, n, num_rows, dim):
@@ -148,40 +150,40 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None)
     Ids equal to ``padding_idx`` are left out."""
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
-    ids, g, dim, dtype, gt, wt = _grad_args(ids, grad, num_rows, dtype)
+    ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
     n = ids.numel()
     ws = None if n <= _FEW_IDS else _grad_workspace(grad, n, num_rows, dim)
     dw = grad.new_empty((num_rows, dim), dtype=dtype)
-    _store_module().embedding_grad(grad.device.index, dw.data_ptr(), wt, dim, num_rows, dim, g.data_ptr(), gt,
+    _store_module().embedding_grad(device, dw.data_ptr(), wt, dim, num_rows, dim, g.data_ptr(), gt,
                                    g.stride(0), ids.data_ptr(), ids.element_size(), n, pad, scale,
-                                   *_span(ws), _stream(grad.device))
+                                   *_span(ws), _raw_stream(device))
     return dw
 
 
 def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None):
     """The gradient of ``embedding`` as its distinct rows: ``(rows, values)``,
     the ids that occur (ascending, int64; without ``padding_idx``) and for each
-    the row ``embedding_grad`` would hold. Waits for the stream once, for the
-    number of rows, so it cannot be captured into a graph."""
+    the row ``embedding_grad`` would hold. Waits once, for the number of
+    rows, so it cannot be captured into a graph."""
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
-    ids, g, dim, dtype, gt, wt = _grad_args(ids, grad, num_rows, dtype)
-    m, dev, stream = _store_module(), grad.device, _stream(grad.device)
+    ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
+    m, stream = _store_module(), _raw_stream(device)
     n = ids.numel()
     most = min(n, num_rows)
     if n <= _FEW_IDS and most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
         rows = grad.new_empty(most, dtype=torch.int64)
         values = grad.new_empty((most, dim), dtype=dtype)
-        count = m.embedding_grad_distinct(dev.index, rows.data_ptr(), values.data_ptr(), wt, dim, most, num_rows, dim,
+        count = m.embedding_grad_distinct(device, rows.data_ptr(), values.data_ptr(), wt, dim, most, num_rows, dim,
                                           g.data_ptr(), gt, g.stride(0), ids.data_ptr(), ids.element_size(), n, pad,
                                           scale, 0, 0, stream)
         return rows.resize_(count), values.resize_(count, dim)
     ws = _grad_workspace(grad, n, num_rows, dim)
-    count = m.embedding_group(dev.index, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
+    count = m.embedding_group(device, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
                               ws.numel(), 0, stream)
     rows = grad.new_empty(count, dtype=torch.int64)
     values = grad.new_empty((count, dim), dtype=dtype)
-    m.embedding_grad_rows(dev.index, rows.data_ptr(), values.data_ptr(), wt, dim, count, num_rows, dim, g.data_ptr(),
+    m.embedding_grad_rows(device, rows.data_ptr(), values.data_ptr(), wt, dim, count, num_rows, dim, g.data_ptr(),
                           gt, g.stride(0), n, scale, ws.data_ptr(), ws.numel(), stream)
     return rows, values
 
@@ -296,7 +298,7 @@ def _span(ws):
 
 def _layer_norm_forward(x, weight, bias, eps, stats):
     dim, xt, pt = _params(x, weight, bias)
-    _need_cuda(x.device, weight, bias)
+    device = _device_of(x, weight, bias)
     rows = _as_rows(x, dim)
     n = rows.shape[0]
     y = _new_like(x)
@@ -304,8 +306,8 @@ def _layer_norm_forward(x, weight, bias, eps, stats):
     if stats:
         mean = x.new_empty(n, dtype=torch.float32)
         rstd = x.new_empty(n, dtype=torch.float32)
-    _store_module().layer_norm(x.device.index, y.data_ptr(), dim, _ptr(mean), _ptr(rstd), rows.data_ptr(), xt,
-                               rows.stride(0), _ptr(weight), _ptr(bias), pt, n, dim, eps, _stream(x.device))
+    _store_module().layer_norm(device, y.data_ptr(), dim, _ptr(mean), _ptr(rstd), rows.data_ptr(), xt,
+                               rows.stride(0), _ptr(weight), _ptr(bias), pt, n, dim, eps, _raw_stream(device))
     return y, mean, rstd
 
 
@@ -323,7 +325,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
         pt = _TYPES[ptype]
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError(f"grad must be like x: {tuple(x.shape)} {x.dtype}, not {tuple(grad.shape)} {grad.dtype}")
-    _need_cuda(x.device, grad, mean, rstd, weight)
+    device = _device_of(x, grad, mean, rstd, weight)
     xr, gr = _as_rows(x, dim), _as_rows(grad, dim)
     n = xr.shape[0]
     for name, s in (("mean", mean), ("rstd", rstd)):
@@ -332,12 +334,13 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
     m = _store_module()
     few = dim <= 4096 and n * max(dim, 128) <= _FEW_NORM  # no workspace
     dx = _new_like(x) if need[0] else None
-    dw = x.new_empty(dim, dtype=ptype) if need[1] else None
-    db = x.new_empty(dim, dtype=ptype) if need[2] else None
+    like = weight if weight is not None else x.new_empty(0, dtype=ptype)
+    dw = like.new_empty(dim) if need[1] else None
+    db = like.new_empty(dim) if need[2] else None
     ws = None if few or not (need[1] or need[2]) else x.new_empty(m.layer_norm_grad_workspace(n, dim), dtype=torch.uint8)
-    m.layer_norm_grad(x.device.index, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
+    m.layer_norm_grad(device, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
                       gr.stride(0), xr.data_ptr(), xt, xr.stride(0), _ptr(weight), pt, mean.data_ptr(),
-                      rstd.data_ptr(), n, dim, *_span(ws), _stream(x.device))
+                      rstd.data_ptr(), n, dim, *_span(ws), _raw_stream(device))
     return dx, dw, db
 
 

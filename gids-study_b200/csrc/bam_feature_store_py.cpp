@@ -501,7 +501,7 @@ PYBIND11_MODULE(BAM_Feature_Store, m) {
       py::arg("id_bytes"), py::arg("n"), py::arg("padding_idx") = -1, py::arg("scale") = 1.0f,
       py::arg("workspace") = 0, py::arg("workspace_bytes") = 0, py::arg("stream") = 0,
       py::call_guard<py::gil_scoped_release>());
-  // returns the number of distinct rows (waits for the stream) unless count_dev is given
+  // returns the number of distinct rows (waits for it) unless count_dev is given
   m.def(
       "embedding_group",
       [](int device, uint64_t ids, int id_bytes, int64_t n, int64_t num_rows, int64_t padding_idx, int64_t dim,
@@ -527,7 +527,7 @@ PYBIND11_MODULE(BAM_Feature_Store, m) {
       py::arg("capacity"), py::arg("num_rows"), py::arg("dim"), py::arg("grad"), py::arg("grad_type"),
       py::arg("grad_stride"), py::arg("n"), py::arg("scale"), py::arg("workspace"), py::arg("workspace_bytes"),
       py::arg("stream") = 0, py::call_guard<py::gil_scoped_release>());
-  // both in one call; returns the number of distinct rows (waits for the stream)
+  // both in one call; returns the number of distinct rows (waits for it)
   m.def(
       "embedding_grad_distinct",
       [](int device, uint64_t rows, uint64_t values, int value_type, int64_t values_stride, int64_t capacity,

@@ -497,9 +497,9 @@ GIDS_API int gids_embedding_grad_rows(int device, int64_t *rows, void *values, i
 
 /* Both in one call, for results that have room for all the rows there can be
  * (capacity at least min(n, num_rows)): nothing waits between the sort and the
- * sums, and up to GIDS_FEW_IDS ids take one kernel. Waits for the stream at the end and
- * returns the number of rows in count_host (refused with GIDS_E_STATE on a stream
- * that is being captured). */
+ * sums, and up to GIDS_FEW_IDS ids take one kernel. Waits for the number of
+ * rows and returns it in count_host (refused with GIDS_E_STATE on a stream that
+ * is being captured); the rows follow in the order of the stream. */
 GIDS_API int gids_embedding_grad_distinct(int device, int64_t *rows, void *values, int value_type,
                                           int64_t values_stride, int64_t capacity, int64_t num_rows, int64_t dim,
                                           const void *grad, int grad_type, int64_t grad_stride, const void *ids,
