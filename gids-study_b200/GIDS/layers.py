@@ -171,14 +171,16 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     m, stream = _store_module(), _raw_stream(device)
     n = ids.numel()
     most = min(n, num_rows)
-    if n <= _FEW_IDS and most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
+    ws = None if n <= _FEW_IDS else _grad_workspace(grad, n, num_rows, dim)
+    if most * dim * dtype.itemsize <= _ONE_CALL_BYTES:
         rows = grad.new_empty(most, dtype=torch.int64)
         values = grad.new_empty((most, dim), dtype=dtype)
         count = m.embedding_grad_distinct(device, rows.data_ptr(), values.data_ptr(), wt, dim, most, num_rows, dim,
                                           g.data_ptr(), gt, g.stride(0), ids.data_ptr(), ids.element_size(), n, pad,
-                                          scale, 0, 0, stream)
+                                          scale, *_span(ws), stream)
         return rows.resize_(count), values.resize_(count, dim)
-    ws = _grad_workspace(grad, n, num_rows, dim)
+    if ws is None:
+        ws = _grad_workspace(grad, n, num_rows, dim)
     count = m.embedding_group(device, ids.data_ptr(), ids.element_size(), n, num_rows, pad, dim, ws.data_ptr(),
                               ws.numel(), 0, stream)
     rows = grad.new_empty(count, dtype=torch.int64)
@@ -188,11 +190,10 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     return rows, values
 
 
-# Up to _FEW_IDS ids one kernel finds the distinct ids and sums their rows, so one call with room
-# for every row there can be is quicker (8 ids x 128 fp32: 27 us a pass instead of 34); with
-# more ids it is not (7,910 x 448 bf16: 49 us, in two calls 43), and the wait for the count
-# lets the result hold no more than the rows there are. Nor should one call take much room.
-_ONE_CALL_BYTES = 8 << 20
+# Results up to this size get room for every row there can be, so that one call sorts and
+# sums without a gap between (7,910 ids x 448 bf16: 32 us a pass instead of 37; 200,000 x 128
+# fp32: 83 instead of 92); larger ones wait for the count and hold no more than the rows there are.
+_ONE_CALL_BYTES = 1 << 28
 
 
 class _Embedding(torch.autograd.Function):
