@@ -376,8 +376,8 @@ __device__ __forceinline__ unsigned int rank_step(SortShared<THREADS>& s, int ra
   return total;
 }
 
-// Stable scatter of tile blockIdx.x by one digit.
-template <int THREADS>
+// Stable scatter of tile blockIdx.x by one digit, ITEMS words a thread at a time.
+template <int THREADS, int ITEMS>
 __global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
                                                                unsigned long long* __restrict__ out, ZeroFill zero) {
   extern __shared__ uint4 dyn[];
@@ -396,9 +396,10 @@ __global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
     const auto load = [&](unsigned int step) {
 #pragma unroll
       for (int k = 0; k < SORT_ITEMS; k++) {
-        const unsigned int i = step + warp * (32 * SORT_ITEMS) + k * 32 + lane;
-        word[k] = i < hi ? source_word(src, i) : 0ull;
-        digit[k] = i < hi ? (unsigned int)(word[k] >> p.shift) & (radix - 1) : 0xffffffffu;
+        const unsigned int i = step + warp * (32 * ITEMS) + k * 32 + lane;
+        const bool in = k < ITEMS && i < hi;
+        word[k] = in ? source_word(src, i) : 0ull;
+        digit[k] = in ? (unsigned int)(word[k] >> p.shift) & (radix - 1) : 0xffffffffu;
       }
     };
     load(lo);
@@ -430,9 +431,9 @@ __global__ void __launch_bounds__(THREADS) scatter_kernel(IdSource src, Pass p,
       s.before[tid] = early;
     }
     digit_bases(s, radix, all);
-    for (unsigned int step = lo; step < hi; step += (THREADS * SORT_ITEMS)) {
+    for (unsigned int step = lo; step < hi; step += THREADS * ITEMS) {
       if (step != lo) load(step);
-      const unsigned int total = rank_step(s, radix, SORT_ITEMS, digit, rank);
+      const unsigned int total = rank_step(s, radix, ITEMS, digit, rank);
 #pragma unroll
       for (int k = 0; k < SORT_ITEMS; k++) {
         if (digit[k] == 0xffffffffu) continue;
@@ -1217,9 +1218,13 @@ void chain(bool first, void (*kernel)(P...), unsigned int grid, unsigned int blo
 bool wide_sort(uint64_t n) { return n > (uint64_t)MAX_TILES * 512 * SORT_ITEMS; }
 constexpr uint64_t SMALL_LIST = (uint64_t)CLUSTER_BLOCKS * CLUSTER_THREADS * SORT_ITEMS;  // for one cluster
 
+// Words of a thread in a step of a scatter: one where that leaves a block to an
+// SM (33,000 ids of 23 bits, sort alone: 32 us, 40 with four; 131,072: 43 and 39).
+int sort_items(uint64_t n) { return n <= (uint64_t)MAX_TILES * 512 ? 1 : SORT_ITEMS; }
+
 // tiles and words per tile of the sort of n words
 void sort_shape(uint64_t n, unsigned int* tiles, unsigned int* per) {
-  const uint64_t threads = wide_sort(n) ? 1024 : 512, step = threads * SORT_ITEMS;
+  const uint64_t threads = wide_sort(n) ? 1024 : 512, step = threads * sort_items(n);
   const uint64_t want = std::min<uint64_t>(MAX_TILES, (n + step - 1) / step);
   const uint64_t p = ((n + want - 1) / want + threads - 1) / threads * threads;
   *per = (unsigned int)p;
@@ -1236,7 +1241,7 @@ uint64_t sorted_at(uint64_t n, uint64_t num_rows, const Workspace& lay) {
 
 // Sorts the ids into the workspace, writes `zero` meanwhile and, if asked,
 // ranks and counts the runs.
-template <int THREADS>
+template <int THREADS, int ITEMS>
 void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks,
                  unsigned long long* count, unsigned long long* host_count, int sms, cudaStream_t st) {
   unsigned int* rank = reinterpret_cast<unsigned int*>(ws + lay.rank);
@@ -1272,7 +1277,7 @@ void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay
     pass.shift += pass.bits;
     pass.bits = (32 + key_bits - pass.shift + (passes - p) - 1) / (passes - p);
     chain(p == 0, count_kernel<THREADS>, grid, THREADS, 0, st, src, pass, next_share());
-    chain(false, scatter_kernel<THREADS>, grid, THREADS,
+    chain(false, scatter_kernel<THREADS, ITEMS>, grid, THREADS,
           sizeof(SortShared<THREADS>) + 16 + 2 * 16 * THREADS, st, src, pass, buf[p & 1], next_share());
     src.id_bytes = 0;
     src.words = buf[p & 1];
@@ -1287,9 +1292,11 @@ void sort_ids_by(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay
 void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, ZeroFill zero, bool ranks,
               unsigned long long* count, unsigned long long* host_count, int sms, cudaStream_t st) {
   if (wide_sort(n))
-    sort_ids_by<1024>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
+    sort_ids_by<1024, SORT_ITEMS>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
+  else if (sort_items(n) == 1)
+    sort_ids_by<512, 1>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
   else
-    sort_ids_by<512>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
+    sort_ids_by<512, SORT_ITEMS>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
 }
 
 template <typename G, typename W, int VEC>

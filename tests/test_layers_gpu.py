@@ -1006,3 +1006,16 @@ def test_norm_gradient_without_a_workspace(layers, n, d):
         wide = torch.zeros(n, d + 3, dtype=x.dtype, device=DEV)
         wide[:, 1:d + 1] = x
         check_norm_grad(layers, wide[:, 1:d + 1], w, g, mean, rstd)
+
+
+@pytest.mark.parametrize("n", [32768, 32769, 33280, 75775, 75776, 75777, 303104, 303105])
+def test_sort_shapes(layers, n):
+    """Around the lengths where the sort changes its kernels and what a thread takes."""
+    for rows in (7, 70000, 1 << 22):
+        ids, g = randint(rows, (n,), seed=n), randn(n, 4, seed=3)
+        r, v = layers.embedding_grad_rows(ids, g, rows, 1.0, 3)
+        want, inv = torch.unique(ids, return_inverse=True)
+        s, a, c = group_sums(inv, g, len(want))
+        keep = want != 3
+        assert torch.equal(r, want[keep])
+        close(v, s[keep], grad_error(a, c, 1.0, s)[keep])
