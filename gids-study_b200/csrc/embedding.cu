@@ -662,13 +662,18 @@ __global__ void __launch_bounds__(256) zero_kernel(ZeroFill z) {
 // A team of lanes walks a chunk of the sorted words for one slab of columns (16
 // bytes of the gradient's row to a lane), with the running sum in registers,
 // and stores a row of the result where the id changes. Rows of the gradient
-// arrive through a ring of asynchronous copies, SEG_DEPTH - 1 rows ahead, which
+// arrive through a ring of asynchronous copies, some rows ahead, which
 // keeps about 128 KB an SM in flight at few registers. Sums of runs that cross
 // the chunks of a block meet in shared memory; those that cross blocks are left
 // in the workspace for join_kernel.
 constexpr int SEG_THREADS = 256;
 constexpr unsigned int SEG_MAX_ROWS = 1024;  // words of a block
-constexpr int SEG_DEPTH = 8;  // rows of the ring, a power of two (4: as fast; 16: 10 to 20 % slower, fewer blocks fit)
+// Rows of the ring, a power of two (with one vector a thread, 4 are as fast; 16
+// are 10 to 20 % slower, as fewer blocks fit), and the ring's bytes.
+__host__ __device__ constexpr int seg_depth(int vec, int k) { return vec > 1 && k == 2 ? 4 : 8; }
+__host__ __device__ constexpr int seg_ring_bytes(int vec, int k, int teams) {
+  return seg_depth(vec, k) * 16 * (vec == 1 ? SEG_THREADS + teams : SEG_THREADS * k);
+}
 
 struct SegArgs {
   const unsigned long long* words;  // sorted
@@ -689,9 +694,9 @@ __device__ __forceinline__ unsigned int key_of(const SegArgs& a, unsigned int i)
   return (unsigned int)(a.words[i] >> 32);
 }
 
-// A thread has K vectors of VEC columns (16 bytes of the gradient), vector k at
-// column first + k * step: one vector where rows are aligned to it, else
-// single elements.
+// A thread has K vectors of VEC columns, vector k at column first + k * step: one
+// or two of 16 bytes of the gradient where rows are aligned to them, else single
+// elements of 16 bytes together.
 template <int VEC, int K>
 struct Columns {
   long long first;
@@ -741,11 +746,17 @@ __device__ __forceinline__ void store_partial(const SegArgs& a, const Columns<VE
 template <typename G, typename W, int VEC, int K>
 __global__ void __launch_bounds__(SEG_THREADS, 4) segment_kernel(SegArgs a) {
   constexpr bool STAGED = VEC == 1;  // a team copies the 16-byte pieces that cover its columns
-  constexpr int P = VEC * K / 2, D = SEG_DEPTH;
+  constexpr int P = VEC * K / 2, D = seg_depth(VEC, K);
   constexpr unsigned int NONE = 0xffffffffu;
   enum : unsigned char { CONT = 1, WHOLE = 2, TAIL = 4 };
+  constexpr bool WIDE = VEC > 1 && K == 2;
   extern __shared__ uint4 ring[];
-  __shared__ unsigned long long words[SEG_MAX_ROWS + 2];  // of the block, with the one before and the one behind
+  // the words of the block, with the one before and the one behind; behind the
+  // ring in the wide kernel (378,383 ids x 5440 fp16: 658 us, 693 in an array)
+  __shared__ unsigned long long word_array[WIDE ? 1 : SEG_MAX_ROWS + 2];
+  unsigned long long* words = word_array;
+  if constexpr (WIDE)
+    words = reinterpret_cast<unsigned long long*>(reinterpret_cast<char*>(ring) + seg_ring_bytes(VEC, K, 0));
   __shared__ F2 heads[P][SEG_THREADS];                    // sums of the runs that chunks start inside
   // CONT: the chunk starts inside a run; WHOLE: and the run goes on behind it;
   // TAIL: a run that starts in the chunk goes on behind it
@@ -767,12 +778,14 @@ __global__ void __launch_bounds__(SEG_THREADS, 4) segment_kernel(SegArgs a) {
   const Columns<VEC, K> c(a, slab);
   const unsigned long long* mine = words + 1 + me * a.chunk;
   // ring slots: a thread's own vector, or its team's row of the slab
-  const int pitch = STAGED ? (SEG_THREADS + (int)teams) * 16 : SEG_THREADS * 16;
+  const int pitch = STAGED ? (SEG_THREADS + (int)teams) * 16 : K * SEG_THREADS * 16;
   char* slot0 = reinterpret_cast<char*>(ring) + (STAGED ? me * (a.team + 1) * 16 : threadIdx.x * 16);
   const char* g0 = reinterpret_cast<const char*>(a.grad) + (STAGED ? c.first - lane : c.first) * (long long)sizeof(G);
   const long long row_bytes = a.grad_stride * (long long)sizeof(G);
   const int slab_bytes = (int)min((long long)a.team * 16, (a.dim - (c.first - (STAGED ? lane : 0))) * (long long)sizeof(G));
   const bool active = STAGED || c.first < a.dim;
+  bool also = false;  // the second vector
+  if constexpr (!STAGED && K == 2) also = c.col(1) < a.dim;
   const auto fetch = [&](unsigned int i) {
     if (i < a.chunk) {
       const unsigned long long w = mine[i];
@@ -785,6 +798,9 @@ __global__ void __launch_bounds__(SEG_THREADS, 4) segment_kernel(SegArgs a) {
             copy_async_tail(dst + q, src - early + q, min(16, early + slab_bytes - q));
         } else {
           copy_async(dst, src, true);
+          if constexpr (K == 2) {
+            if (also) copy_async(dst + SEG_THREADS * 16, src + a.team * 16, true);
+          }
         }
       }
     }
@@ -817,7 +833,8 @@ __global__ void __launch_bounds__(SEG_THREADS, 4) segment_kernel(SegArgs a) {
                         ? *reinterpret_cast<const G*>(src + early + (k * a.team + lane) * (int)sizeof(G))
                         : from_f32<G>(0.0f);
     } else {
-      v[0] = *reinterpret_cast<const RowVec<G, VEC>*>(src);
+#pragma unroll
+      for (int k = 0; k < K; k++) v[k] = *reinterpret_cast<const RowVec<G, VEC>*>(src + k * SEG_THREADS * 16);
     }
 #pragma unroll
     for (int p = 0; p < P; p++) acc[p] = add2(acc[p], pair_of(v, p));
@@ -1299,6 +1316,16 @@ void sort_ids(const IdSource& ids, uint64_t n, char* ws, const Workspace& lay, Z
     sort_ids_by<512, SORT_ITEMS>(ids, n, ws, lay, zero, ranks, count, host_count, sms, st);
 }
 
+template <typename G, typename W, int VEC, int K>
+void launch_segments_k(SegArgs a, const SegPlan& p, bool first, cudaStream_t st) {
+  const uint64_t grid = (uint64_t)p.blocks * a.slabs;
+  GIDS_CHECK(grid < (1ull << 31), GIDS_E_UNSUPPORTED, "too many rows x columns for one launch");
+  const size_t smem = seg_ring_bytes(VEC, K, SEG_THREADS / (int)p.team) +
+                      (VEC > 1 && K == 2 ? (p.rows + 2) * sizeof(unsigned long long) : 0);
+  chain(first, segment_kernel<G, W, VEC, K>, (unsigned int)grid, SEG_THREADS, smem, st, a);
+  if (p.blocks > 1) chain(false, join_kernel<W, VEC, K>, (unsigned int)grid, SEG_THREADS, 0, st, a);
+}
+
 template <typename G, typename W, int VEC>
 void launch_segments(SegArgs a, bool first, cudaStream_t st) {
   const SegPlan p = seg_plan(a.n, (uint64_t)a.dim, sizeof(G));
@@ -1306,12 +1333,20 @@ void launch_segments(SegArgs a, bool first, cudaStream_t st) {
   a.slabs = p.slabs;
   a.chunk = p.chunk;
   a.blocks = p.blocks;
-  const uint64_t grid = (uint64_t)p.blocks * p.slabs;
-  GIDS_CHECK(grid < (1ull << 31), GIDS_E_UNSUPPORTED, "too many rows x columns for one launch");
-  constexpr int K = 16 / (VEC * (int)sizeof(G));
-  const size_t smem = (size_t)SEG_DEPTH * 16 * (SEG_THREADS + (VEC == 1 ? SEG_THREADS / p.team : 0));
-  chain(first, segment_kernel<G, W, VEC, K>, (unsigned int)grid, SEG_THREADS, smem, st, a);
-  if (p.blocks > 1) chain(false, join_kernel<W, VEC, K>, (unsigned int)grid, SEG_THREADS, 0, st, a);
+  if constexpr (VEC > 1) {
+    // Two vectors a thread, where that leaves every SM eight blocks: the work on
+    // a row's word serves twice the columns. (The sums are bound by instructions
+    // else: 378,383 ids x 5440 fp16, dense, 775 us by one vector a thread, 658 by two.
+    // With four blocks to an SM, 131,072 x 1024 bf16, both take 78 us.)
+    const unsigned int half = (p.slabs + 1) / 2;
+    if (p.slabs > 1 && (uint64_t)p.blocks * half >= 148 * 8) {
+      a.slabs = half;
+      return launch_segments_k<G, W, VEC, 2>(a, p, first, st);
+    }
+    launch_segments_k<G, W, VEC, 1>(a, p, first, st);
+  } else {
+    launch_segments_k<G, W, 1, 16 / (int)sizeof(G)>(a, p, first, st);
+  }
 }
 
 template <typename G, typename W>

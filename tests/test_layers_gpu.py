@@ -1019,3 +1019,13 @@ def test_sort_shapes(layers, n):
         keep = want != 3
         assert torch.equal(r, want[keep])
         close(v, s[keep], grad_error(a, c, 1.0, s)[keep])
+
+
+@pytest.mark.parametrize("dim,t", [(4096, "f16"), (4104, "bf16"), (2052, "f32"), (5120, "bf16")])
+def test_sums_of_long_rows_over_many_ids(layers, dim, t):
+    """Two vectors a thread: whole teams, and teams that end in the first or the second vector."""
+    n = 40001
+    for rows in (30, 30000):
+        ids = randint(rows, (n,), seed=dim)
+        ids[: n // 3] = rows // 2  # a run over many blocks
+        check_grad(layers, ids, randn(n, dim, seed=1, dtype=t), rows, 0.5, 1)
