@@ -4,7 +4,7 @@
 // EMB_UNROLL vectors of a flat (row, vector) index space, so rows of any width
 // fill the warps; an id outside the table gives a zero row and sets the device's
 // error word. Rows that are not aligned to vectors come through shared memory
-// instead. Bound by HBM: 1,000,003 rows of 768 fp16 take 504 us, 0.94 of the
+// instead. Bound by HBM: 1,000,003 rows of 768 fp16 take 507 us, 0.94 of the
 // measured copy rate for the 3.07 GB they read and write (545 us when the output
 // stays in L2 and pushes out rows of the table).
 //
@@ -1391,7 +1391,8 @@ void launch_tiny_vec(const TinyArgs& a, const Rows& out, const Rows& grad, int s
   launch_tiny<G, W, 1>(a, sms, st);
 }
 
-// (64 ids into 5,000 x 128 fp32, dense: 16 us a pass by the sorted list, 12 this way.)
+// (64 ids into 5,000 x 128 fp32, dense: 16 us a pass by the sorted list, 12 this
+// way, and 9 since it needs no workspace.)
 void tiny(const TinyArgs& a, const Rows& out, const Rows& grad, int sms, cudaStream_t st) {
   if (out.type == GIDS_F32) {
     if (grad.type == GIDS_F32) return launch_tiny_vec<float, float>(a, out, grad, sms, st);
