@@ -333,12 +333,14 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
         if s.dtype != torch.float32 or s.numel() != n or not s.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 tensor of {n} elements")
     m = _store_module()
-    few = dim <= 4096 and n * max(dim, 128) <= _FEW_NORM  # no workspace
+    few = dim <= 4096 and n * max(dim, 128) <= _FEW_NORM
     dx = _new_like(x) if need[0] else None
     like = weight if weight is not None else x.new_empty(0, dtype=ptype)
     dw = like.new_empty(dim) if need[1] else None
     db = like.new_empty(dim) if need[2] else None
-    ws = None if few or not (need[1] or need[2]) else x.new_empty(m.layer_norm_grad_workspace(n, dim), dtype=torch.uint8)
+    ws = None  # few rows, and dx alone, need none
+    if not few and (need[1] or need[2]):
+        ws = x.new_empty(m.layer_norm_grad_workspace(n, dim), dtype=torch.uint8)
     m.layer_norm_grad(device, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
                       gr.stride(0), xr.data_ptr(), xt, xr.stride(0), _ptr(weight), pt, mean.data_ptr(),
                       rstd.data_ptr(), n, dim, *_span(ws), _raw_stream(device))

@@ -1095,7 +1095,8 @@ __global__ void __launch_bounds__(TINY_THREADS) tiny_grad_kernel(TinyArgs a) {
   W* table = reinterpret_cast<W*>(a.out);
   const auto clear_span = [&](W* out, long long left) {
     if constexpr (VEC == 1) {  // the elements before the first boundary of 16 bytes
-      const int head = (int)min((long long)((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / (int)sizeof(W), left);
+      const int early = (int)(-reinterpret_cast<uintptr_t>(out) & 15) / (int)sizeof(W);
+      const int head = (int)min((long long)early, left);
       if ((int)lane < head) out[lane] = from_f32<W>(0.0f);
       out += head;
       left -= head;
