@@ -510,7 +510,8 @@ GIDS_API int gids_embedding_grad_distinct(int device, int64_t *rows, void *value
  * sqrt(v + eps), v the mean squared difference from m, of row i. weight and
  * bias (dim elements of param_type, which is x's type or GIDS_F32) may be NULL
  * (1 and 0). mean and rstd (n float32 each, both or neither NULL) receive m
- * and r for the gradient. y may be x (same address and stride). */
+ * and r for the gradient. y may be x (same address and stride). A row whose sum
+ * is out of float32's range gives NaN. */
 GIDS_API int gids_layer_norm(int device, void *y, int64_t y_stride, float *mean, float *rstd, const void *x,
                              int x_type, int64_t x_stride, const void *weight, const void *bias, int param_type,
                              int64_t n, int64_t dim, float eps, void *stream);
@@ -518,7 +519,8 @@ GIDS_API int gids_layer_norm(int device, void *y, int64_t y_stride, float *mean,
  * mean and rstd it stored: dx (x's type), dweight = the sum of grad * xh and
  * dbias = the sum of grad over the rows (param_type), xh = (x - mean) * rstd;
  * each may be NULL (not wanted). dx may be grad or x (same address and
- * stride). The workspace is needed for dweight and dbias. */
+ * stride). The workspace is needed for dweight and dbias (small calls apart,
+ * see GIDS_FEW_NORM). */
 GIDS_API int gids_layer_norm_grad_workspace(int64_t n, int64_t dim, uint64_t *bytes);
 GIDS_API int gids_layer_norm_grad(int device, void *dx, int64_t dx_stride, void *dweight, void *dbias,
                                   const void *grad, int64_t grad_stride, const void *x, int x_type, int64_t x_stride,

@@ -1029,3 +1029,14 @@ def test_sums_of_long_rows_over_many_ids(layers, dim, t):
         ids = randint(rows, (n,), seed=dim)
         ids[: n // 3] = rows // 2  # a run over many blocks
         check_grad(layers, ids, randn(n, dim, seed=1, dtype=t), rows, 0.5, 1)
+
+
+def test_few_ids_next_to_one_another(layers):
+    """Named rows at the ends of the stretches that are zeroed together, and side by side."""
+    for dim, rows in ((1, 1000), (4, 640), (64, 40), (600, 9)):
+        step = max(1, min(128, 2048 // (4 * dim)))
+        at = [r for b in range(0, rows, step) for r in (b, b + 1, b + step - 1) if r < rows][:127] + [rows - 1]
+        check_grad(layers, torch.tensor(at, device=DEV), randn(len(at), dim, seed=dim), rows, 1.0)
+    ids = torch.arange(128, device=DEV)
+    check_grad(layers, ids, randn(128, 2, seed=1), 128, 1.0)
+    check_grad(layers, ids + 3, randn(128, 2, seed=1), 400, 1.0, 5)
