@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(256) zero_kernel(ZeroFill z) {
 }
 
 // ------------------------------------------------------------ sums over runs
-// A team of lanes walks a chunk of the sorted words for one slab of columns (16
+// A team of lanes walks a chunk of the sorted words for one slab of columns (16 or 32
 // bytes of the gradient's row to a lane), with the running sum in registers,
 // and stores a row of the result where the id changes. Rows of the gradient
 // arrive through a ring of asynchronous copies, some rows ahead, which
