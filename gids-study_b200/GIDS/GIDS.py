@@ -422,7 +422,7 @@ class GIDS:
 
         batch = self.window_buffer.pop(0)
         if self.heterograph:
-            ret_ten, outs, idxs, ns, keys = {}, [], [], [], []
+            ret_ten, outs, idxs, ns, keys, keep_alive = {}, [], [], [], [], []
             for key, v in batch[0].items():
                 if key in self.node_embeddings:
                     ret_ten[key] = None  # looked up when the batch is handed out
@@ -431,6 +431,7 @@ class GIDS:
                     ret_ten[key] = self._new_out(0, dim)
                     continue
                 g_index = _as_index(v, self.device)
+                keep_alive.append(g_index)  # else the next type's copy may take its memory before the launch
                 out = self._new_out(len(g_index), dim)
                 ret_ten[key] = out
                 outs.append(out.data_ptr())
@@ -438,6 +439,7 @@ class GIDS:
                 ns.append(len(g_index))
                 keys.append(self._key_off(key))
             self.BAM_FS.read_feature_hetero(len(outs), outs, idxs, ns, dim, self.cache_dim, keys, stream)
+            del keep_alive  # stream-ordered: safe to release once the launch is queued
             self.GIDS_time += time.time() - GIDS_time_start
             return self._hand_out(batch, ret_ten)
 

@@ -200,3 +200,14 @@ def test_static_hot_set_through_gids(table):
     n_hot_refs = sum(int(np.isin(b[0].numpy(), list(hot_set)).sum()) for b in bs)
     assert st["read_io"] == st0["read_io"] and hits >= n_hot_refs > 0  # nothing new inserted, pinned rows hit
     g.close()
+
+
+def test_heterograph_types_of_one_size(table):
+    """Ids on the host, the same number for every type: each type's copy on the GPU is of one size."""
+    g = make_gids(table, heterograph=True, heterograph_map=hmap())
+    rng = np.random.default_rng(12)
+    bs = [[{t: torch.as_tensor(rng.integers(0, size, size=500), dtype=torch.int32) for t, size in TYPES.items()}, f"s{i}"]
+          for i in range(3)]
+    got = run(g, bs, 3, CDIM)
+    check_hetero(table, got, [[{t: v.long() for t, v in b[0].items()}, b[1]] for b in bs], CDIM)
+    g.close()

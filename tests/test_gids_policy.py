@@ -344,3 +344,32 @@ def test_store_tensor_passes_rows(fake):
     t = torch.zeros((5, 1024))
     g.store_tensor(t, 0)
     assert ("store_tensor", t.data_ptr(), 5, 0) in g.BAM_FS.calls
+
+
+@pytest.mark.parametrize("accumulator", [False, True])
+def test_heterograph_ids_outlive_the_launch(fake, monkeypatch, accumulator):
+    """Ids that had to be copied (another type, another device) stay allocated until the launch of all
+    node types is queued: the memory of a copy that is let go earlier may hold the next type's ids."""
+    import weakref
+
+    copies = []
+
+    def as_index(v, device):
+        t = v.to(torch.int64).clone()
+        copies.append(weakref.ref(t))
+        return t
+
+    monkeypatch.setattr(gmod, "_as_index", as_index)
+    hmap = {"paper": 0, "author": 400, "fos": 700}
+    g = fake(heterograph=True, heterograph_map=hmap, accumulator_flag=accumulator)
+    alive = []
+    name = "read_feature_merged_hetero" if accumulator else "read_feature_hetero"
+    read = getattr(g.BAM_FS, name)
+    setattr(g.BAM_FS, name, lambda *a: (alive.extend(r() is not None for r in copies), read(*a)))
+    rng = np.random.default_rng(4)
+    b = [{k: torch.as_tensor(rng.integers(0, 300, 25), dtype=torch.int32) for k in hmap}, "s", "bl"]
+    feats = g.fetch_feature(64, iter([b]), "cpu")[-1]
+    assert alive == [True] * 3
+    for k, off in hmap.items():
+        assert np.array_equal(feats[k].numpy(), oracle.gather(FakeStore.table, b[0][k].numpy().astype(np.int64),
+                                                              key_off=off))
