@@ -16,7 +16,8 @@ bit. Workspaces come from torch's allocator for each call, so calls on several
 streams and in several captured graphs share nothing.
 
 An id outside its table gives a zero row and no gradient, and raises at the next
-embedding call on that device, or at ``check_ids``. A backward pass that is
+embedding call on that device, or at ``check_ids``. Derivatives are reverse-mode:
+inputs with a forward-mode tangent are refused. A backward pass that is
 captured into a CUDA graph must not meet an eager graph of the same parameters
 that is still alive (torch's rule for every op): drop eager losses and outputs first.
 """
@@ -25,6 +26,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from .sampler import _store_module as _import_module
 
@@ -61,6 +63,15 @@ def _device_of(first: torch.Tensor, *others) -> int:
         if t is not None and t.get_device() != device:
             raise ValueError(f"a tensor is on {t.device}, the others on {first.device}")
     return device
+
+
+def _check_forward_ad(*tensors):
+    """The operators have no forward-mode derivative: refuse inputs that carry a
+    tangent, which autograd would drop without a word where none of them requires grad."""
+    if _forward_ad._current_level >= 0:  # inside a dual_level
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("GIDS.layers has no forward-mode derivatives (an input carries a tangent)")
 
 
 def _check_ids(ids: torch.Tensor) -> torch.Tensor:
@@ -148,6 +159,7 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None)
     ``scale`` times the sum of the rows of ``grad`` whose id is v (in position
     order, in float32), rounded to ``dtype`` (grad's by default, or float32).
     Ids equal to ``padding_idx`` are left out."""
+    _check_forward_ad(grad)
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
     ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
@@ -165,6 +177,7 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     the ids that occur (ascending, int64; without ``padding_idx``) and for each
     the row ``embedding_grad`` would hold. Waits once, for the number of
     rows, so it cannot be captured into a graph."""
+    _check_forward_ad(grad)
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
     ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
@@ -222,6 +235,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, sparse=False, dtype=None
     ``weight``: rows of ``padding_idx`` get no gradient, and with ``sparse`` the
     gradient is a coalesced sparse tensor of the distinct rows (for
     torch.optim.SparseAdam and the like) instead of a dense table."""
+    _check_forward_ad(weight)
     dtype = weight.dtype if dtype is None else dtype
     scale = float(scale)
     if padding_idx is not None:
@@ -318,6 +332,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
     ``layer_norm_stats`` returns them). ``need`` says which are wanted (None for
     the others). dweight and dbias have weight's type; without a weight,
     ``param_dtype`` (x's by default, or float32)."""
+    _check_forward_ad(grad, x, mean, rstd, weight)
     dim, xt, pt = _params(x, weight, None)
     ptype = weight.dtype if weight is not None else param_dtype or x.dtype
     if weight is None:
@@ -366,6 +381,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of ``x``: ``(x - mean) / sqrt(var +
     eps) * weight + bias`` in x's type; weight and bias [dim] are of x's type or
     float32, or None. Differentiable in all three."""
+    _check_forward_ad(x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, float(eps))
@@ -375,6 +391,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def layer_norm_stats(x, weight=None, bias=None, eps=1e-5):
     """``(y, mean, rstd)``: ``layer_norm`` (without autograd) and the float32
     statistics of every row that ``layer_norm_grad`` takes."""
+    _check_forward_ad(x, weight, bias)
     return _layer_norm_forward(x, weight, bias, float(eps), True)
 
 
