@@ -17,7 +17,9 @@ streams and in several captured graphs share nothing.
 
 An id outside its table gives a zero row and no gradient, and raises at the next
 embedding call on that device, or at ``check_ids``. Derivatives are reverse-mode:
-inputs with a forward-mode tangent are refused. A backward pass that is
+inputs with a forward-mode tangent are refused. ``embedding`` and ``layer_norm``
+can be traced by torch.jit.trace (for a replay in Python); what else records
+torch operations is refused. A backward pass that is
 captured into a CUDA graph must not meet an eager graph of the same parameters
 that is still alive (torch's rule for every op): drop eager losses and outputs first.
 """
@@ -72,6 +74,22 @@ def _check_forward_ad(*tensors):
         for t in tensors:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError("GIDS.layers has no forward-mode derivatives (an input carries a tangent)")
+
+
+_tracing_state = torch._C._get_tracing_state  # None unless torch.jit.trace is at work
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def _check_recording(what=None):
+    """A recording of torch operations (make_fx, and torch.jit.trace where the
+    call cannot record itself) sees a kernel's empty result but not the kernel: refused."""
+    if what is not None and _tracing_state() is not None:
+        raise RuntimeError(f"{what} cannot be traced by torch.jit.trace")
+    if _dispatch_modes():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            raise RuntimeError("GIDS.layers cannot be recorded by make_fx")
 
 
 def _check_ids(ids: torch.Tensor) -> torch.Tensor:
@@ -160,6 +178,7 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None)
     order, in float32), rounded to ``dtype`` (grad's by default, or float32).
     Ids equal to ``padding_idx`` are left out."""
     _check_forward_ad(grad)
+    _check_recording("embedding_grad")
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
     ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
@@ -178,6 +197,7 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     the row ``embedding_grad`` would hold. Waits once, for the number of
     rows, so it cannot be captured into a graph."""
     _check_forward_ad(grad)
+    _check_recording("embedding_grad_rows")
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
     ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
@@ -236,11 +256,13 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, sparse=False, dtype=None
     gradient is a coalesced sparse tensor of the distinct rows (for
     torch.optim.SparseAdam and the like) instead of a dense table."""
     _check_forward_ad(weight)
+    _check_recording()
     dtype = weight.dtype if dtype is None else dtype
     scale = float(scale)
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
-    if weight.requires_grad and torch.is_grad_enabled():
+    # a trace records the function, whose replay runs the kernel
+    if (weight.requires_grad and torch.is_grad_enabled()) or _tracing_state() is not None:
         return _Embedding.apply(ids, weight, scale, padding_idx, bool(sparse), dtype)
     return _embedding_forward(ids, weight, scale, dtype)
 
@@ -333,6 +355,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
     the others). dweight and dbias have weight's type; without a weight,
     ``param_dtype`` (x's by default, or float32)."""
     _check_forward_ad(grad, x, mean, rstd, weight)
+    _check_recording("layer_norm_grad")
     dim, xt, pt = _params(x, weight, None)
     ptype = weight.dtype if weight is not None else param_dtype or x.dtype
     if weight is None:
@@ -382,8 +405,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     eps) * weight + bias`` in x's type; weight and bias [dim] are of x's type or
     float32, or None. Differentiable in all three."""
     _check_forward_ad(x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    _check_recording()
+    if _tracing_state() is not None or (
+            torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                         or (bias is not None and bias.requires_grad))):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm_forward(x, weight, bias, float(eps), False)[0]
 
@@ -392,6 +417,7 @@ def layer_norm_stats(x, weight=None, bias=None, eps=1e-5):
     """``(y, mean, rstd)``: ``layer_norm`` (without autograd) and the float32
     statistics of every row that ``layer_norm_grad`` takes."""
     _check_forward_ad(x, weight, bias)
+    _check_recording("layer_norm_stats")
     return _layer_norm_forward(x, weight, bias, float(eps), True)
 
 

@@ -129,3 +129,61 @@ def test_a_gradient_with_a_tangent_is_refused(layers):
             g = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(out, leaf, g)
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_traced_modules_run_their_kernels(layers, requires_grad, grad_mode):
+    emb, norm = layers.NodeEmbedding(5, 8, scale=2.0), layers.LayerNorm(8)
+    model = torch.nn.Sequential(emb, norm).requires_grad_(requires_grad)
+    with torch.set_grad_enabled(grad_mode):
+        traced = torch.jit.trace(model, (IDS,))
+        before = layers.kernels.calls
+        other = torch.tensor([4, 4, 1, 3])
+        got = traced(other)
+        assert layers.kernels.calls == before + 2
+        want = torch.nn.functional.layer_norm(2.0 * emb.weight[other], (8,), norm.weight, norm.bias)
+        torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-4)
+        assert got.requires_grad == (requires_grad and grad_mode)
+
+
+def test_what_a_recording_would_miss_is_refused(layers):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    w, x, st = torch.randn(5, 8), torch.randn(4, 8), torch.ones(4)
+    calls = (lambda t: layers.embedding_grad(IDS, t, 5), lambda t: layers.embedding_grad_rows(IDS, t, 5)[1],
+             lambda t: layers.layer_norm_grad(t, x, st, st)[0], lambda t: layers.layer_norm_stats(t)[0])
+    for call in calls:
+        with pytest.raises(RuntimeError, match="jit.trace"):
+            torch.jit.trace(call, (x,))
+    for call in (*calls, lambda t: layers.layer_norm(t), lambda t: layers.embedding(IDS, t)):
+        for requires_grad in (False, True):
+            with pytest.raises(RuntimeError, match="make_fx"):
+                make_fx(call)(x.clone().requires_grad_(requires_grad))
+            for mode in ("fake", "symbolic"):
+                with pytest.raises(RuntimeError):
+                    make_fx(call, tracing_mode=mode)(x.clone().requires_grad_(requires_grad))
+    # other modes see the operations and leave the call as it is
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    want = layers.layer_norm(x)
+    with Watch():
+        assert torch.equal(layers.layer_norm(x), want) and torch.equal(layers.embedding(IDS, w), w[IDS])
+
+
+def test_transforms_of_functions_are_refused(layers):
+    w, x = torch.randn(5, 8), torch.randn(4, 8)
+    for call in (lambda: torch.vmap(lambda i: layers.embedding(i, w))(IDS),
+                 lambda: torch.vmap(lambda t: layers.embedding(IDS, t))(torch.randn(2, 5, 8)),
+                 lambda: torch.vmap(layers.layer_norm)(torch.randn(2, 4, 8)),
+                 lambda: torch.func.jvp(layers.layer_norm, (x,), (x,)),
+                 lambda: torch.func.jvp(lambda t: layers.embedding(IDS, t), (w,), (w,)),
+                 lambda: torch.func.grad(lambda t: layers.layer_norm(t).sum())(x),
+                 lambda: torch.func.grad(lambda t: layers.embedding(IDS, t).sum())(w),
+                 lambda: torch.export.export(layers.LayerNorm(8), (x,))):
+        with pytest.raises(Exception):
+            call()
