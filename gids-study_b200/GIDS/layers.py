@@ -17,7 +17,7 @@ streams and in several captured graphs share nothing.
 
 An id outside its table gives a zero row and no gradient, and raises at the next
 embedding call on that device, or at ``check_ids``. Derivatives are reverse-mode:
-inputs with a forward-mode tangent are refused. ``embedding`` and ``layer_norm``
+inputs with a forward-mode tangent are refused, and so are second derivatives. ``embedding`` and ``layer_norm``
 can be traced by torch.jit.trace (for a replay in Python); what else records
 torch operations is refused. A backward pass that is
 captured into a CUDA graph must not meet an eager graph of the same parameters
@@ -25,6 +25,7 @@ that is still alive (torch's rule for every op): drop eager losses and outputs f
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -229,6 +230,40 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
 _ONE_CALL_BYTES = 1 << 28
 
 
+class _Underivable(torch.autograd.Function):
+    """Hands on gradients that depend on ``inputs`` and refuses to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, grads, *inputs):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradients of GIDS.layers have no derivative (second derivatives are not supported)")
+
+
+def _first_derivative(backward):
+    """A backward pass of kernels that autograd does not see. Where a graph of it is
+    asked for (create_graph), the gradients stay tied to what they depend on, so that
+    a second derivative is an error: torch's once_differentiable leaves them
+    untied, and torch.autograd.functional.hvp and hessian then take it as zero."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, grad):
+        with torch.no_grad():
+            out = backward(ctx, grad)
+        if not torch.is_grad_enabled():
+            return out
+        at = [i for i, t in enumerate(out) if t is not None]
+        tied = _Underivable.apply(tuple(out[i] for i in at), grad, *ctx.saved_tensors)
+        out = list(out)
+        for i, t in zip(at, tied):
+            out[i] = t
+        return tuple(out)
+
+    return wrapper
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, sparse, dtype):
@@ -237,7 +272,7 @@ class _Embedding(torch.autograd.Function):
         return _embedding_forward(ids, weight, scale, dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
         num_rows, scale, padding_idx, sparse, dtype = ctx.conf
@@ -394,7 +429,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, grad):
         x, mean, rstd, weight = ctx.saved_tensors
         return *layer_norm_grad(grad, x, mean, rstd, weight, ctx.needs_input_grad[:3], ctx.bias_type), None

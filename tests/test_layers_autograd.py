@@ -187,3 +187,31 @@ def test_transforms_of_functions_are_refused(layers):
                  lambda: torch.export.export(layers.LayerNorm(8), (x,))):
         with pytest.raises(Exception):
             call()
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_second_derivatives_are_refused(layers, sparse):
+    x, w = torch.randn(4, 8), torch.randn(5, 8)
+    p = torch.ones(8)
+    losses = [(lambda t: layers.layer_norm(t).square().sum(), x), (lambda t: layers.layer_norm(x, t).square().sum(), p),
+              (lambda t: layers.layer_norm(x, p, t).pow(3).sum(), torch.zeros(8)),
+              (lambda t: layers.embedding(IDS, t, 2.0, sparse=sparse).pow(3).sum(), w)]
+    for loss, at in losses:
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.functional.hvp(loss, at, torch.ones_like(at))
+        if not sparse:
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.functional.hessian(loss, at)
+        leaf = at.clone().requires_grad_()
+        (g,) = torch.autograd.grad(loss(leaf), leaf, create_graph=True)
+        (want,) = torch.autograd.grad(loss(leaf), leaf)
+        assert torch.equal(g.detach().to_dense(), want.to_dense()) and g.is_sparse == want.is_sparse
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (g.to_dense() if g.is_sparse else g).square().sum().backward()
+        loss(leaf).backward(create_graph=True)  # a graph that nobody differentiates
+        assert torch.equal(leaf.grad.detach().to_dense(), want.to_dense())
+        leaf.grad = None
+    # what does not depend on the gradient is no one's second derivative
+    leaf = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(layers.layer_norm(leaf).sum(), leaf)
+    assert not g.requires_grad
