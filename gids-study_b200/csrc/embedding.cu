@@ -1439,6 +1439,18 @@ void launch_embedding_vec(const EmbArgs& a, const Rows& out, const Rows& weight,
   GIDS_CUDA(cudaGetLastError());
 }
 
+// A new word of mapped host memory, and its address on the device.
+template <typename T>
+T* mapped_word(T** dev) {
+  RelaxedCapture any;
+  T* host = nullptr;
+  GIDS_CUDA(cudaHostAlloc(&host, sizeof(T), cudaHostAllocMapped | cudaHostAllocPortable));
+  const cudaError_t e = cudaHostGetDevicePointer(dev, host, 0);
+  if (e != cudaSuccess) cudaFreeHost(host);
+  GIDS_CUDA(e);
+  return host;
+}
+
 // A word of mapped host memory for the time of a call that waits for a number
 // from its kernels. They store it once, as soon as they know it, so the call
 // returns while they still work (500,009 ids x 128 fp32: 171 us a pass by waiting
@@ -1458,10 +1470,11 @@ struct HostWord {
         g_words.pop_back();
       }
     }
-    if (!host)
-      GIDS_CUDA(cudaHostAlloc(&host, sizeof(*host), cudaHostAllocMapped | cudaHostAllocPortable));
+    if (host)
+      GIDS_CUDA(cudaHostGetDevicePointer(&dev, host, 0));
+    else
+      host = mapped_word(&dev);
     __atomic_store_n(host, NONE, __ATOMIC_RELEASE);
-    GIDS_CUDA(cudaHostGetDevicePointer(&dev, host, 0));
   }
   unsigned long long wait(cudaStream_t st) {
     unsigned long long v = NONE;
@@ -1472,6 +1485,7 @@ struct HostWord {
       v = __atomic_load_n(host, __ATOMIC_ACQUIRE);
     }
     if (v == NONE) {
+      RelaxedCapture any;
       GIDS_CUDA(cudaStreamSynchronize(st));
       v = __atomic_load_n(host, __ATOMIC_ACQUIRE);
     }
@@ -1520,17 +1534,9 @@ void allow_smem(const void* kernel, size_t bytes) {
 int* id_error_word(int device) {
   std::lock_guard<std::mutex> lk(g_err_mu);
   if (!g_err_dev[device]) {
-    // allocation is allowed while the calling thread captures a stream: the
-    // word is not part of the graph
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    GIDS_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-    int* h = nullptr;
-    cudaError_t e = cudaHostAlloc(&h, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    GIDS_CUDA(e);
-    *h = 0;
     int* d = nullptr;
-    GIDS_CUDA(cudaHostGetDevicePointer(&d, h, 0));
+    int* h = mapped_word(&d);
+    *h = 0;
     g_err_dev[device] = d;
     g_err_host[device].store(h, std::memory_order_release);
   }
@@ -1765,7 +1771,10 @@ void embedding_check(int device, cudaStream_t st) {
   GIDS_CUDA(cudaStreamIsCapturing(st, &cap));
   GIDS_CHECK(cap == cudaStreamCaptureStatusNone, GIDS_E_STATE,
              "the check waits for the stream, which is being captured into a graph");
-  GIDS_CUDA(cudaStreamSynchronize(st));
+  {
+    RelaxedCapture any;
+    GIDS_CUDA(cudaStreamSynchronize(st));
+  }
   check_id_errors(device);
 }
 

@@ -53,6 +53,18 @@ struct DeviceGuard {
   }
 };
 
+// RAII: while another thread captures a stream in the global mode (torch's
+// default), calls such as an allocation or a wait are forbidden to every thread
+// and spoil that capture. They are open to a thread in the relaxed mode, which is
+// right for what is not part of any graph.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { GIDS_CUDA(cudaThreadExchangeStreamCaptureMode(&mode)); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  RelaxedCapture(const RelaxedCapture&) = delete;
+  RelaxedCapture& operator=(const RelaxedCapture&) = delete;
+};
+
 // -------------------------------------------------------- page state word
 // One 64-bit word per page of the range (the page table). It plays the role
 // of the reference's data_page_t state word (page_cache_backup.h:104-117,

@@ -1040,3 +1040,55 @@ def test_few_ids_next_to_one_another(layers):
     ids = torch.arange(128, device=DEV)
     check_grad(layers, ids, randn(128, 2, seed=1), 128, 1.0)
     check_grad(layers, ids + 3, randn(128, 2, seed=1), 400, 1.0, 5)
+
+
+CAPTURE_BESIDE = """
+import threading
+import torch
+from GIDS import layers
+
+DEV = "cuda:0"
+s = torch.cuda.Stream()
+ids = torch.arange(100, device=DEV) % 40
+g = torch.randn(100, 16, device=DEV)
+x = torch.randn(64, 32, device=DEV)
+with torch.cuda.stream(s):  # kernels and the allocator's blocks, but no call that returns a count yet
+    dense = layers.embedding_grad(ids, g, 50)
+    room = [torch.empty(50, dtype=torch.int64, device=DEV), torch.empty(50, 16, device=DEV)]
+    del room
+y = layers.layer_norm(x)
+torch.cuda.synchronize()
+got, bad = [], []
+
+def other():
+    try:
+        with torch.cuda.stream(s):
+            got.append(layers.embedding_grad_rows(ids, g, 50))
+            layers.check_ids(DEV)
+    except Exception as e:
+        bad.append(repr(e))
+
+gr = torch.cuda.CUDAGraph()
+with torch.cuda.graph(gr):
+    z = layers.layer_norm(x)
+    t = threading.Thread(target=other)
+    t.start()
+    t.join()
+assert not bad, bad
+gr.replay()
+torch.cuda.synchronize()
+assert torch.equal(z, y)
+rows, values = got[0]
+assert torch.equal(rows, torch.arange(40, device=DEV)) and torch.equal(values, dense[:40])
+"""
+
+
+def test_counting_rows_beside_another_threads_capture(layers):
+    """The first call that returns a count, while another thread captures a graph in torch's default mode."""
+    import os
+    import subprocess
+    import sys
+
+    run = subprocess.run([sys.executable, "-c", CAPTURE_BESIDE], capture_output=True, text=True, timeout=300,
+                         env={**os.environ, "PYTHONPATH": os.pathsep.join(p for p in sys.path if p)})
+    assert run.returncode == 0, run.stderr[-2000:]
