@@ -350,7 +350,11 @@ struct RowRing {
 // The rounded mean is off by up to half a step of the mean, which is not small
 // beside the differences when the mean is large against them. `off` is the
 // mean of the differences from it: the second pass takes it out again.
-__device__ __forceinline__ float variance(float mean_sq, float off) { return fmaxf(mean_sq - off * off, 0.0f); }
+// (Not fmaxf, which would turn the NaN of a row with NaN or infinities into 0.)
+__device__ __forceinline__ float variance(float mean_sq, float off) {
+  const float v = mean_sq - off * off;
+  return v < 0.0f ? 0.0f : v;
+}
 
 // blockDim = (threads of a group, groups).
 template <typename X, int VEC, int K, int R, int STAGES, int MODE, int THREADS, int GROUP>

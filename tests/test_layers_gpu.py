@@ -1092,3 +1092,24 @@ def test_counting_rows_beside_another_threads_capture(layers):
     run = subprocess.run([sys.executable, "-c", CAPTURE_BESIDE], capture_output=True, text=True, timeout=300,
                          env={**os.environ, "PYTHONPATH": os.pathsep.join(p for p in sys.path if p)})
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [1, 8, 33, 768, 1001, 4096, 20000])
+def test_norm_statistics_of_rows_that_are_not_finite(layers, d, t):
+    """NaN or infinities anywhere in a row make its mean (or, for infinities, at least its variance) NaN: rstd
+    is NaN with it, and the rows beside it keep their bits."""
+    x = randn(9, d, seed=d, dtype=t)
+    want = layers.layer_norm_stats(x)
+    x[1, d // 2] = float("nan")
+    x[4, 0] = float("inf")
+    x[7, d - 1] = -float("inf")
+    x[7, d // 3] = float("inf") if d > 1 else -float("inf")
+    y, mean, rstd = layers.layer_norm_stats(x)
+    ref = (x.double() - x.double().mean(1, keepdim=True)).square().mean(1)
+    bad = torch.isnan(ref)
+    assert bad.tolist() == [i in (1, 4, 7) for i in range(9)]
+    assert torch.equal(torch.isnan(rstd), bad) and bool(torch.isnan(y[bad]).all())
+    assert not bool(torch.isfinite(mean[bad]).any())
+    for a, b in zip((y, mean, rstd), want):
+        assert torch.equal(bits(a[~bad]), bits(b[~bad]))
