@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import math
 import time
+from collections.abc import Mapping
 
 import torch
 
@@ -73,6 +74,11 @@ def _with_features(batch, feat):
     return batch
 
 
+def _by_type(norm) -> bool:
+    """Whether feature_norm holds a norm for each node type, rather than one for all."""
+    return isinstance(norm, (Mapping, torch.nn.ModuleDict))  # a ModuleDict is not a Mapping
+
+
 class GIDS:
     """Feature fetcher over the GPU page cache (GIDS.py:490-1128).
 
@@ -114,8 +120,8 @@ class GIDS:
     differentiable in their parameters. ``node_embeddings`` (heterographs; a
     dict of node type -> ``layers.NodeEmbedding``) names the types that have no
     stored features: their rows come from the learnable table instead of the
-    store. ``feature_norm`` (a ``layers.LayerNorm``, or in a heterograph a dict
-    of node type -> one) normalises the rows of the batch. Both run when the
+    store. ``feature_norm`` (a ``layers.LayerNorm``, or in a heterograph a dict or
+    ``torch.nn.ModuleDict`` of node type -> one) normalises the rows of the batch. Both run when the
     batch is handed out, so with the accumulator they see the parameters of
     that step, not those of the gather.
     """
@@ -128,7 +134,7 @@ class GIDS:
                  node_embeddings=None, feature_norm=None):
         if node_embeddings and not heterograph:
             raise ValueError("node_embeddings are for the node types of a heterograph (heterograph=True)")
-        if isinstance(feature_norm, dict) and not heterograph:
+        if _by_type(feature_norm) and not heterograph:
             raise ValueError("feature_norm by node type needs a heterograph (heterograph=True)")
         self.node_embeddings = dict(node_embeddings or {})
         self.feature_norm = feature_norm
@@ -396,7 +402,7 @@ class GIDS:
             for key, table in self.node_embeddings.items():
                 if key in feat:
                     feat[key] = table(_as_index(batch[0][key], self.device))
-        if isinstance(self.feature_norm, dict):
+        if _by_type(self.feature_norm):
             feat = {k: self.feature_norm[k](v) if k in self.feature_norm else v for k, v in feat.items()}
         elif self.feature_norm is not None:
             feat = {k: self.feature_norm(v) for k, v in feat.items()} if self.heterograph else self.feature_norm(feat)

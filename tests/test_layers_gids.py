@@ -1,6 +1,8 @@
 """GIDS.fetch_feature with the model's input layers (node_embeddings,
 feature_norm): which rows are gathered, marked and looked up, on the CPU
 against a fake store."""
+import types
+
 import numpy as np
 import pytest
 import torch
@@ -113,3 +115,37 @@ def test_accumulator_with_nothing_stored_takes_one_batch_at_a_time(fake):  # noq
         out = g.fetch_feature(64, it, "cpu")
         assert out[1] == b[1] and torch.equal(out[-1]["author"], t.rows[b[0]["author"]])
     assert len(t.seen) == 5
+
+
+class Plus(torch.nn.Module):
+    def __init__(self, by):
+        super().__init__()
+        self.by = by
+
+    def forward(self, x):
+        return x + self.by
+
+
+@pytest.mark.parametrize("accumulator", [False, True])
+def test_norms_in_a_module_dict(fake, accumulator):  # noqa: F811
+    """The way a model registers its norms by node type."""
+    t = Table(100, 64)
+    norms = torch.nn.ModuleDict({"paper": Plus(1.0), "author": Plus(2.0)})
+    g = fake(heterograph=True, heterograph_map=MAP, node_embeddings={"author": t}, feature_norm=norms,
+             accumulator_flag=accumulator)
+    bs = hetero(2, seed=8)
+    it = iter([list(b) for b in bs])
+    f = g.fetch_feature(64, it, "cpu")[-1]
+    assert np.array_equal(f["paper"].numpy(), expect(bs[0][0]["paper"]) + 1)
+    assert torch.equal(f["author"], t.rows[bs[0][0]["author"]] + 2)
+    assert np.array_equal(f["fos"].numpy(), expect(bs[0][0]["fos"], 600))
+    norms["fos"] = Plus(3.0)  # the loader holds the model's dict, not a copy
+    f = g.fetch_feature(64, it, "cpu")[-1]
+    assert np.array_equal(f["fos"].numpy(), expect(bs[1][0]["fos"], 600) + 3)
+    h = hetero(1)[0]
+    g = fake(heterograph=True, heterograph_map=MAP, feature_norm=types.MappingProxyType({"paper": Plus(1.0)}))
+    f = g.fetch_feature(64, iter([list(h)]), "cpu")[-1]
+    assert np.array_equal(f["paper"].numpy(), expect(h[0]["paper"]) + 1)
+    for typed in (norms, types.MappingProxyType({"paper": Plus(1.0)})):
+        with pytest.raises(ValueError, match="heterograph"):
+            fake(feature_norm=typed)
