@@ -123,7 +123,10 @@ class GIDS:
     store. ``feature_norm`` (a ``layers.LayerNorm``, or in a heterograph a dict or
     ``torch.nn.ModuleDict`` of node type -> one) normalises the rows of the batch. Both run when the
     batch is handed out, so with the accumulator they see the parameters of
-    that step, not those of the gather.
+    that step, not those of the gather. If they raise (an embedding reports ids of
+    an earlier call, of whatever thread, by raising in the next one), the
+    gathered batch is not lost: the next ``fetch_feature`` hands it out, and
+    gives it up only if they raise again.
     """
 
     def __init__(self, page_size=4096, off=0, cache_dim=1024, num_ele=300 * 1000 * 1000 * 1024, num_ssd=1,
@@ -138,6 +141,7 @@ class GIDS:
             raise ValueError("feature_norm by node type needs a heterograph (heterograph=True)")
         self.node_embeddings = dict(node_embeddings or {})
         self.feature_norm = feature_norm
+        self._held = None  # a gathered batch whose input layers raised
         if dtype is None:
             dtype = torch.int64 if long_type else torch.float32
         if dtype not in _STORE_CLASSES:
@@ -314,6 +318,7 @@ class GIDS:
                     self.BAM_FS.unset_window_buffering(t.data_ptr(), len(t), key, stream)
         self.window_buffer.clear()
         self.return_torch_buffer.clear()
+        self._held = None
         self.wb_init = False
 
     def _batch_ids(self, batch):
@@ -396,9 +401,19 @@ class GIDS:
             print("Cannot find key: ", key, " in the heterograph map!")
         return 0
 
-    def _hand_out(self, batch, feat):
+    def _hand_out(self, batch, feat, again=False):
         """The batch with its features, after the model's input layers (extension)."""
+        try:
+            done = self._input_layers(batch, feat)
+        except Exception:
+            if not again:
+                self._held = (batch, feat)
+            raise
+        return _with_features(batch, done)
+
+    def _input_layers(self, batch, feat):
         if self.node_embeddings:
+            feat = dict(feat)
             for key, table in self.node_embeddings.items():
                 if key in feat:
                     feat[key] = table(_as_index(batch[0][key], self.device))
@@ -406,10 +421,13 @@ class GIDS:
             feat = {k: self.feature_norm[k](v) if k in self.feature_norm else v for k, v in feat.items()}
         elif self.feature_norm is not None:
             feat = {k: self.feature_norm(v) for k, v in feat.items()} if self.heterograph else self.feature_norm(feat)
-        return _with_features(batch, feat)
+        return feat
 
     def fetch_feature(self, dim, it, device):
         """Next batch from ``it`` with its gathered features appended (GIDS.py:791-1058)."""
+        if self._held is not None:
+            (batch, feat), self._held = self._held, None
+            return self._hand_out(batch, feat, again=True)
         GIDS_time_start = time.time()
         stream = _current_stream_handle(self.device)
         self._wb_dim = dim

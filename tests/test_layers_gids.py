@@ -149,3 +149,55 @@ def test_norms_in_a_module_dict(fake, accumulator):  # noqa: F811
     for typed in (norms, types.MappingProxyType({"paper": Plus(1.0)})):
         with pytest.raises(ValueError, match="heterograph"):
             fake(feature_norm=typed)
+
+
+class Reports(Table):
+    """Raises in the calls named, as the table's lookup does for ids of an earlier call."""
+
+    def __init__(self, rows, dim, at):
+        super().__init__(rows, dim)
+        self.at = at
+
+    def __call__(self, ids):
+        if len(self.seen) in self.at:
+            self.seen.append(None)
+            raise RuntimeError("an id of an earlier embedding call lay outside its table")
+        return super().__call__(ids)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(window_buffer=True, wb_size=2), dict(accumulator_flag=True)],
+                         ids=lambda kw: next(iter(kw), "plain"))
+def test_a_report_loses_no_batch(fake, kw):  # noqa: F811
+    t = Reports(100, 8, {1, 3})
+    g = fake(heterograph=True, heterograph_map=MAP, node_embeddings={"author": t}, **kw)
+    g.required_accesses = 100
+    bs = hetero(9, seed=5)
+    it = iter([list(b) for b in bs])
+    got, raised = [], 0
+    while len(got) < 4:
+        try:
+            got.append(g.fetch_feature(64, it, "cpu"))
+        except RuntimeError:
+            raised += 1
+    assert raised == 2
+    for out, b in zip(got, bs):
+        assert out[1] == b[1] and torch.equal(out[-1]["author"], t.rows[b[0]["author"]])
+        assert np.array_equal(out[-1]["paper"].numpy(), expect(b[0]["paper"]))
+        assert len(out) == 4
+
+
+def test_a_batch_that_raises_twice_is_given_up(fake):  # noqa: F811
+    t = Reports(100, 8, {0, 1})
+    g = fake(heterograph=True, heterograph_map=MAP, node_embeddings={"author": t})
+    bs = hetero(2, seed=6)
+    it = iter([list(b) for b in bs])
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="earlier"):
+            g.fetch_feature(64, it, "cpu")
+    assert g.fetch_feature(64, it, "cpu")[1] == bs[1][1]
+    g = fake(heterograph=True, heterograph_map=MAP, node_embeddings={"author": Reports(100, 8, {0})})
+    it = iter([list(b) for b in bs])
+    with pytest.raises(RuntimeError):
+        g.fetch_feature(64, it, "cpu")
+    g.drop_window_buffer()  # nothing of the old window is left
+    assert g.fetch_feature(64, it, "cpu")[1] == bs[1][1]
