@@ -1696,6 +1696,7 @@ void embedding_group(int device, const void* ids, int id_bytes, int64_t n, int64
                      int64_t dim, void* ws, uint64_t ws_bytes, uint64_t* count_dev, uint64_t* count_host,
                      cudaStream_t st) {
   check_group(device, ids, id_bytes, n, num_rows, padding_idx, dim, ws, ws_bytes, false);
+  GIDS_CHECK(((uintptr_t)count_dev) % 8 == 0, GIDS_E_INVAL, "count_dev: address not aligned to its element");
   check_id_errors(device);
   DeviceGuard dg(device);
   if (count_host) check_not_capturing(st);

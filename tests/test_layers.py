@@ -197,3 +197,13 @@ def test_few_constants_match_the_header(built):
     text = (pathlib.Path(gids_abi.__file__).parents[1] / "include" / "gids_b200.h").read_text()
     assert int(re.search(r"#define GIDS_FEW_IDS (\d+)", text)[1]) == layers._FEW_IDS
     assert eval(re.search(r"#define GIDS_FEW_NORM (.+)", text)[1]) == layers._FEW_NORM
+
+
+def test_abi_refuses_an_unaligned_count(built):
+    """The kernels store the number of rows as one 64-bit word."""
+    L = abi()
+    for off in (1, 2, 4):
+        a = [0, P, 8, 4, 10, -1, 8, P, 1 << 30, P + off, None, None]
+        assert L.gids_embedding_group(*a) == GIDS_E_INVAL, off
+    a = [0, None, 8, 0, 10, -1, 8, P, 1 << 30, P + 4, None, None]  # no ids: still set
+    assert L.gids_embedding_group(*a) == GIDS_E_INVAL
