@@ -68,29 +68,34 @@ def _device_of(first: torch.Tensor, *others) -> int:
     return device
 
 
-def _check_forward_ad(*tensors):
-    """The operators have no forward-mode derivative: refuse inputs that carry a
-    tangent, which autograd would drop without a word where none of them requires grad."""
-    if _forward_ad._current_level >= 0:  # inside a dual_level
-        for t in tensors:
-            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("GIDS.layers has no forward-mode derivatives (an input carries a tangent)")
-
-
-_tracing_state = torch._C._get_tracing_state  # None unless torch.jit.trace is at work
+_is_tracing = torch._C._is_tracing  # by torch.jit.trace
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 
 
-def _check_recording(what=None):
-    """A recording of torch operations (make_fx, and torch.jit.trace where the
-    call cannot record itself) sees a kernel's empty result but not the kernel: refused."""
-    if what is not None and _tracing_state() is not None:
-        raise RuntimeError(f"{what} cannot be traced by torch.jit.trace")
+def _check_transforms(*tensors):
+    """What autograd would not see, or a recording would miss, is refused: for
+    calls inside a forward_ad.dual_level or a dispatch mode (the callers look, as
+    that is all that most calls pay for).
+
+    The operators have no forward-mode derivative, so a tangent would be dropped without a
+    word where no input requires grad. A recording of torch operations (make_fx) sees a
+    kernel's empty result but not the kernel."""
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("GIDS.layers has no forward-mode derivatives (an input carries a tangent)")
     if _dispatch_modes():
         from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
         if get_proxy_mode() is not None:
             raise RuntimeError("GIDS.layers cannot be recorded by make_fx")
+
+
+def _check_transforms_and_trace(what, *tensors):
+    """The same for the operators that torch.jit.trace cannot record as a function of their own."""
+    if _is_tracing():
+        raise RuntimeError(f"{what} cannot be traced by torch.jit.trace")
+    _check_transforms(*tensors)
 
 
 def _check_ids(ids: torch.Tensor) -> torch.Tensor:
@@ -99,16 +104,15 @@ def _check_ids(ids: torch.Tensor) -> torch.Tensor:
     return ids.contiguous()
 
 
-def _as_rows(t: torch.Tensor, dim: int) -> torch.Tensor:
-    """t as a matrix of rows [*, dim] whose columns are consecutive (a view where there is one)."""
-    if t.dim() == 2:
-        if t.is_contiguous():
-            return t
-    else:
+def _as_rows(t: torch.Tensor, dim: int):
+    """t as a matrix of rows [*, dim] whose columns are consecutive (a view where there is one), and its row stride."""
+    if t.dim() != 2:
         t = t.reshape(-1, dim)
+    if t.is_contiguous():  # (asking for this costs less than one stride)
+        return t, dim
     if (dim > 1 and t.stride(1) != 1) or t.stride(0) < 0:
-        t = t.contiguous()
-    return t
+        return t.contiguous(), dim
+    return t, t.stride(0)
 
 
 def _new_like(t: torch.Tensor) -> torch.Tensor:
@@ -139,30 +143,40 @@ def _embedding_forward(ids, weight, scale, dtype):
     if weight.dim() != 2:
         raise ValueError(f"weight must be a matrix, not {tuple(weight.shape)}")
     num_rows, dim = weight.shape
-    wt, ot = _type(weight.dtype, "weight"), _type(dtype, "dtype")
+    wt = ot = _type(weight.dtype, "weight")
+    if dtype is not weight.dtype:
+        ot = _type(dtype, "dtype")
     device = _device_of(weight, ids)
-    if dim > 1 and weight.stride(1) != 1:
-        raise ValueError("the columns of weight must be consecutive (stride 1)")
+    stride = dim
+    if not weight.is_contiguous():
+        stride = weight.stride(0)
+        if dim > 1 and weight.stride(1) != 1:
+            raise ValueError("the columns of weight must be consecutive (stride 1)")
     ids = _check_ids(ids)
     shape = (*ids.shape, dim)
     out = weight.new_empty(shape) if ot == wt else weight.new_empty(shape, dtype=dtype)
     if dim:
         _store_module().embedding(device, out.data_ptr(), ot, dim, weight.data_ptr(), wt,
-                                  weight.stride(0), num_rows, dim, ids.data_ptr(), ids.element_size(), ids.numel(),
+                                  stride, num_rows, dim, ids.data_ptr(), ids.element_size(), ids.numel(),
                                   scale, _raw_stream(device))
     return out
 
 
 def _grad_args(ids, grad, num_rows, dtype):
     ids = _check_ids(ids)
-    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
-        raise ValueError(f"grad {tuple(grad.shape)} does not hold one row for each of the ids {tuple(ids.shape)}")
-    dim = grad.shape[-1]
+    shape = grad.shape
+    if len(shape) < 1 or shape[:-1] != ids.shape:
+        raise ValueError(f"grad {tuple(shape)} does not hold one row for each of the ids {tuple(ids.shape)}")
+    dim = shape[-1]
     if dim < 1:
         raise ValueError("grad has no columns")
-    dtype = grad.dtype if dtype is None else dtype
-    gt, wt = _type(grad.dtype, "grad"), _type(dtype, "dtype")
-    return ids, _as_rows(grad, dim), dim, dtype, gt, wt, _device_of(grad, ids)
+    given = grad.dtype
+    gt = wt = _type(given, "grad")
+    if dtype is None:
+        dtype = given
+    elif dtype is not given:
+        wt = _type(dtype, "dtype")
+    return ids, *_as_rows(grad, dim), dim, dtype, gt, wt, _device_of(grad, ids)
 
 
 def _grad_workspace(grad, n, num_rows, dim):
@@ -178,16 +192,16 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=None)
     ``scale`` times the sum of the rows of ``grad`` whose id is v (in position
     order, in float32), rounded to ``dtype`` (grad's by default, or float32).
     Ids equal to ``padding_idx`` are left out."""
-    _check_forward_ad(grad)
-    _check_recording("embedding_grad")
+    if _forward_ad._current_level >= 0 or _dispatch_modes() or _is_tracing():
+        _check_transforms_and_trace("embedding_grad", grad)
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
-    ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
+    ids, g, stride, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
     n = ids.numel()
     ws = None if n <= _FEW_IDS else _grad_workspace(grad, n, num_rows, dim)
     dw = grad.new_empty((num_rows, dim), dtype=dtype)
     _store_module().embedding_grad(device, dw.data_ptr(), wt, dim, num_rows, dim, g.data_ptr(), gt,
-                                   g.stride(0), ids.data_ptr(), ids.element_size(), n, pad, scale,
+                                   stride, ids.data_ptr(), ids.element_size(), n, pad, scale,
                                    *_span(ws), _raw_stream(device))
     return dw
 
@@ -197,11 +211,11 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     the ids that occur (ascending, int64; without ``padding_idx``) and for each
     the row ``embedding_grad`` would hold. Waits once, for the number of
     rows, so it cannot be captured into a graph."""
-    _check_forward_ad(grad)
-    _check_recording("embedding_grad_rows")
+    if _forward_ad._current_level >= 0 or _dispatch_modes() or _is_tracing():
+        _check_transforms_and_trace("embedding_grad_rows", grad)
     num_rows = int(num_rows)
     pad = _padding(padding_idx, num_rows)
-    ids, g, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
+    ids, g, stride, dim, dtype, gt, wt, device = _grad_args(ids, grad, num_rows, dtype)
     m, stream = _store_module(), _raw_stream(device)
     n = ids.numel()
     most = min(n, num_rows)
@@ -210,7 +224,7 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
         rows = grad.new_empty(most, dtype=torch.int64)
         values = grad.new_empty((most, dim), dtype=dtype)
         count = m.embedding_grad_distinct(device, rows.data_ptr(), values.data_ptr(), wt, dim, most, num_rows, dim,
-                                          g.data_ptr(), gt, g.stride(0), ids.data_ptr(), ids.element_size(), n, pad,
+                                          g.data_ptr(), gt, stride, ids.data_ptr(), ids.element_size(), n, pad,
                                           scale, *_span(ws), stream)
         return rows.resize_(count), values.resize_(count, dim)
     if ws is None:
@@ -220,7 +234,7 @@ def embedding_grad_rows(ids, grad, num_rows, scale=1.0, padding_idx=None, dtype=
     rows = grad.new_empty(count, dtype=torch.int64)
     values = grad.new_empty((count, dim), dtype=dtype)
     m.embedding_grad_rows(device, rows.data_ptr(), values.data_ptr(), wt, dim, count, num_rows, dim, g.data_ptr(),
-                          gt, g.stride(0), n, scale, ws.data_ptr(), ws.numel(), stream)
+                          gt, stride, n, scale, ws.data_ptr(), ws.numel(), stream)
     return rows, values
 
 
@@ -290,14 +304,14 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, sparse=False, dtype=None
     ``weight``: rows of ``padding_idx`` get no gradient, and with ``sparse`` the
     gradient is a coalesced sparse tensor of the distinct rows (for
     torch.optim.SparseAdam and the like) instead of a dense table."""
-    _check_forward_ad(weight)
-    _check_recording()
+    if _forward_ad._current_level >= 0 or _dispatch_modes():
+        _check_transforms(weight)
     dtype = weight.dtype if dtype is None else dtype
     scale = float(scale)
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
     # a trace records the function, whose replay runs the kernel
-    if (weight.requires_grad and torch.is_grad_enabled()) or _tracing_state() is not None:
+    if (weight.requires_grad and torch.is_grad_enabled()) or _is_tracing():
         return _Embedding.apply(ids, weight, scale, padding_idx, bool(sparse), dtype)
     return _embedding_forward(ids, weight, scale, dtype)
 
@@ -336,9 +350,10 @@ class NodeEmbedding(torch.nn.Module):
 # ----------------------------------------------------------------- layer norm
 def _params(x, weight, bias):
     """dim and the type code of weight and bias (x's where there are none)."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must have rows of at least one column, not {tuple(x.shape)}")
-    dim = x.shape[-1]
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"x must have rows of at least one column, not {tuple(shape)}")
+    dim = shape[-1]
     xt = _type(x.dtype, "x")
     pt = None
     for name, p in (("weight", weight), ("bias", bias)):
@@ -346,7 +361,7 @@ def _params(x, weight, bias):
             continue
         if p.shape != (dim,):
             raise ValueError(f"{name} must have shape ({dim},), not {tuple(p.shape)}")
-        if dim > 1 and p.stride(0) != 1:
+        if not p.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         t = _type(p.dtype, name)
         if pt is not None and t != pt:
@@ -371,7 +386,7 @@ def _span(ws):
 def _layer_norm_forward(x, weight, bias, eps, stats):
     dim, xt, pt = _params(x, weight, bias)
     device = _device_of(x, weight, bias)
-    rows = _as_rows(x, dim)
+    rows, stride = _as_rows(x, dim)
     n = rows.shape[0]
     y = _new_like(x)
     mean = rstd = None
@@ -379,7 +394,7 @@ def _layer_norm_forward(x, weight, bias, eps, stats):
         mean = x.new_empty(n, dtype=torch.float32)
         rstd = x.new_empty(n, dtype=torch.float32)
     _store_module().layer_norm(device, y.data_ptr(), dim, _ptr(mean), _ptr(rstd), rows.data_ptr(), xt,
-                               rows.stride(0), _ptr(weight), _ptr(bias), pt, n, dim, eps, _raw_stream(device))
+                               stride, _ptr(weight), _ptr(bias), pt, n, dim, eps, _raw_stream(device))
     return y, mean, rstd
 
 
@@ -389,8 +404,8 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
     ``layer_norm_stats`` returns them). ``need`` says which are wanted (None for
     the others). dweight and dbias have weight's type; without a weight,
     ``param_dtype`` (x's by default, or float32)."""
-    _check_forward_ad(grad, x, mean, rstd, weight)
-    _check_recording("layer_norm_grad")
+    if _forward_ad._current_level >= 0 or _dispatch_modes() or _is_tracing():
+        _check_transforms_and_trace("layer_norm_grad", grad, x, mean, rstd, weight)
     dim, xt, pt = _params(x, weight, None)
     ptype = weight.dtype if weight is not None else param_dtype or x.dtype
     if weight is None:
@@ -400,7 +415,8 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError(f"grad must be like x: {tuple(x.shape)} {x.dtype}, not {tuple(grad.shape)} {grad.dtype}")
     device = _device_of(x, grad, mean, rstd, weight)
-    xr, gr = _as_rows(x, dim), _as_rows(grad, dim)
+    xr, x_stride = _as_rows(x, dim)
+    gr, g_stride = _as_rows(grad, dim)
     n = xr.shape[0]
     for name, s in (("mean", mean), ("rstd", rstd)):
         if s.dtype != torch.float32 or s.numel() != n or not s.is_contiguous():
@@ -415,7 +431,7 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None, need=(True, True, True), p
     if not few and (need[1] or need[2]):
         ws = x.new_empty(m.layer_norm_grad_workspace(n, dim), dtype=torch.uint8)
     m.layer_norm_grad(device, _ptr(dx), dim if need[0] else 0, _ptr(dw), _ptr(db), gr.data_ptr(),
-                      gr.stride(0), xr.data_ptr(), xt, xr.stride(0), _ptr(weight), pt, mean.data_ptr(),
+                      g_stride, xr.data_ptr(), xt, x_stride, _ptr(weight), pt, mean.data_ptr(),
                       rstd.data_ptr(), n, dim, *_span(ws), _raw_stream(device))
     return dx, dw, db
 
@@ -439,9 +455,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of ``x``: ``(x - mean) / sqrt(var +
     eps) * weight + bias`` in x's type; weight and bias [dim] are of x's type or
     float32, or None. Differentiable in all three."""
-    _check_forward_ad(x, weight, bias)
-    _check_recording()
-    if _tracing_state() is not None or (
+    if _forward_ad._current_level >= 0 or _dispatch_modes():
+        _check_transforms(x, weight, bias)
+    if _is_tracing() or (
             torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                          or (bias is not None and bias.requires_grad))):
         return _LayerNorm.apply(x, weight, bias, float(eps))
@@ -451,8 +467,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def layer_norm_stats(x, weight=None, bias=None, eps=1e-5):
     """``(y, mean, rstd)``: ``layer_norm`` (without autograd) and the float32
     statistics of every row that ``layer_norm_grad`` takes."""
-    _check_forward_ad(x, weight, bias)
-    _check_recording("layer_norm_stats")
+    if _forward_ad._current_level >= 0 or _dispatch_modes() or _is_tracing():
+        _check_transforms_and_trace("layer_norm_stats", x, weight, bias)
     return _layer_norm_forward(x, weight, bias, float(eps), True)
 
 
