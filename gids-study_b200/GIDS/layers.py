@@ -16,12 +16,15 @@ bit. Workspaces come from torch's allocator for each call, so calls on several
 streams and in several captured graphs share nothing.
 
 An id outside its table gives a zero row and no gradient, and raises at the next
-embedding call on that device, or at ``check_ids``. Derivatives are reverse-mode:
-inputs with a forward-mode tangent are refused, and so are second derivatives. ``embedding`` and ``layer_norm``
-can be traced by torch.jit.trace (for a replay in Python); what else records
-torch operations is refused. A backward pass that is
-captured into a CUDA graph must not meet an eager graph of the same parameters
-that is still alive (torch's rule for every op): drop eager losses and outputs first.
+embedding call on that device (of any thread and stream; that call did nothing and can
+be repeated), or at ``check_ids``.
+
+Derivatives are reverse-mode and first: inputs with a forward-mode tangent are
+refused, and so are second derivatives. ``embedding`` and ``layer_norm`` can be
+traced by torch.jit.trace (for a replay in Python); what else records torch
+operations is refused. A backward pass that is captured into a CUDA graph must not
+meet an eager graph of the same parameters that is still alive (torch's rule for
+every op): drop eager losses and outputs first.
 """
 from __future__ import annotations
 

@@ -4,7 +4,7 @@
 // EMB_UNROLL vectors of a flat (row, vector) index space, so rows of any width
 // fill the warps; an id outside the table gives a zero row and sets the device's
 // error word. Rows that are not aligned to vectors come through shared memory
-// instead. Bound by HBM: 1,000,003 rows of 768 fp16 take 507 us, 0.94 of the
+// instead. Bound by HBM: 1,000,003 rows of 768 fp16 take 519 us, 0.92 of the
 // measured copy rate for the 3.07 GB they read and write (545 us when the output
 // stays in L2 and pushes out rows of the table).
 //

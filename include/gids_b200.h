@@ -459,8 +459,9 @@ GIDS_API int gids_out_degree(int device, const void *indices, int index_bytes, u
  * num_rows rows. ids: int32 or int64 (id_bytes 4 or 8). out has the table's
  * type, or any type if the table is float32; in the table's type a scale of 1
  * copies the bits. An id outside the table gives a
- * zero row; the next embedding call on the device (before it does anything), or
- * gids_embedding_check, returns GIDS_E_RANGE for it once. */
+ * zero row; the next embedding call on the device (before it does anything; of
+ * whatever thread and stream, so it can be repeated), or gids_embedding_check,
+ * returns GIDS_E_RANGE for it once. */
 GIDS_API int gids_embedding(int device, void *out, int out_type, int64_t out_stride, const void *weight,
                             int weight_type, int64_t weight_stride, int64_t num_rows, int64_t dim, const void *ids,
                             int id_bytes, int64_t n, float scale, void *stream);
@@ -481,7 +482,7 @@ GIDS_API int gids_embedding_grad(int device, void *dweight, int weight_type, int
 /* The same gradient as the distinct rows, for tables too large for a dense
  * one, in two calls. gids_embedding_group sorts the ids into the workspace and
  * counts the distinct ones that are neither padding nor outside the table:
- * count_dev (device, may be NULL) receives the number without a wait;
+ * count_dev (device, 8-byte aligned, may be NULL) receives the number without a wait;
  * count_host (may be NULL) makes the call wait and return it there (refused
  * with GIDS_E_STATE on a stream that is being captured).
  * gids_embedding_grad_rows, with the same n, num_rows, dim and workspace,
@@ -510,8 +511,9 @@ GIDS_API int gids_embedding_grad_distinct(int device, int64_t *rows, void *value
  * sqrt(v + eps), v the mean squared difference from m, of row i. weight and
  * bias (dim elements of param_type, which is x's type or GIDS_F32) may be NULL
  * (1 and 0). mean and rstd (n float32 each, both or neither NULL) receive m
- * and r for the gradient. y may be x (same address and stride). A row whose sum
- * is out of float32's range gives NaN. */
+ * and r for the gradient. y may be x (same address and stride). A row with NaN
+ * or infinities, or whose sum is out of float32's range, gives NaN in y and in
+ * r; one whose squared differences alone sum to more gives r = 0 and y = bias. */
 GIDS_API int gids_layer_norm(int device, void *y, int64_t y_stride, float *mean, float *rstd, const void *x,
                              int x_type, int64_t x_stride, const void *weight, const void *bias, int param_type,
                              int64_t n, int64_t dim, float eps, void *stream);

@@ -1113,3 +1113,17 @@ def test_norm_statistics_of_rows_that_are_not_finite(layers, d, t):
     assert not bool(torch.isfinite(mean[bad]).any())
     for a, b in zip((y, mean, rstd), want):
         assert torch.equal(bits(a[~bad]), bits(b[~bad]))
+
+
+@pytest.mark.parametrize("d", [8, 33, 1024, 20000])
+def test_norm_of_rows_out_of_range(layers, d):
+    """What float32 statistics cannot hold: a sum out of range gives NaN, squares alone out of range rstd = 0."""
+    x, b = randn(4, d, seed=d), randn(d, seed=1)
+    x[1] = 3e38
+    x[2, ::2] = 1e25
+    x[2, 1::2] = -1e25
+    y, mean, rstd = layers.layer_norm_stats(x, None, b)
+    assert bool(torch.isnan(y[1]).all()) and bool(torch.isnan(rstd[1]))
+    assert float(rstd[2]) == 0 and torch.equal(y[2], b) and bool(torch.isfinite(mean[2]))
+    ref, _, _, err = norm_ref(x[[0, 3]], None, b, 1e-5)
+    close(y[[0, 3]], ref, err)
