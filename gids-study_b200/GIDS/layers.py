@@ -267,12 +267,13 @@ def _first_derivative(backward):
 
     @functools.wraps(backward)
     def wrapper(ctx, grad):
+        saved = ctx.saved_tensors  # once: torch.utils.checkpoint allows no second look
         with torch.no_grad():
-            out = backward(ctx, grad)
+            out = backward(ctx, saved, grad)
         if not torch.is_grad_enabled():
             return out
         at = [i for i, t in enumerate(out) if t is not None]
-        tied = _Underivable.apply(tuple(out[i] for i in at), grad, *ctx.saved_tensors)
+        tied = _Underivable.apply(tuple(out[i] for i in at), grad, *saved)
         out = list(out)
         for i, t in zip(at, tied):
             out[i] = t
@@ -290,8 +291,8 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     @_first_derivative
-    def backward(ctx, grad):
-        (ids,) = ctx.saved_tensors
+    def backward(ctx, saved, grad):
+        (ids,) = saved
         num_rows, scale, padding_idx, sparse, dtype = ctx.conf
         if not sparse:
             dw = embedding_grad(ids, grad, num_rows, scale, padding_idx, dtype)
@@ -449,8 +450,8 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     @_first_derivative
-    def backward(ctx, grad):
-        x, mean, rstd, weight = ctx.saved_tensors
+    def backward(ctx, saved, grad):
+        x, mean, rstd, weight = saved
         return *layer_norm_grad(grad, x, mean, rstd, weight, ctx.needs_input_grad[:3], ctx.bias_type), None
 
 

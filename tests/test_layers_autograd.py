@@ -215,3 +215,36 @@ def test_second_derivatives_are_refused(layers, sparse):
     leaf = x.clone().requires_grad_()
     (g,) = torch.autograd.grad(layers.layer_norm(leaf).sum(), leaf)
     assert not g.requires_grad
+
+
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_checkpointed_layers(layers, create_graph):
+    """torch.utils.checkpoint recomputes what the backward pass reads, and lets it be read once."""
+    from torch.utils.checkpoint import checkpoint
+
+    emb, norm = layers.NodeEmbedding(5, 8), layers.LayerNorm(8)
+    out = checkpoint(lambda i: norm(emb(i)), IDS, use_reentrant=False)
+    params = (emb.weight, norm.weight, norm.bias)
+    got = torch.autograd.grad(out.square().sum(), params, create_graph=create_graph)
+    want = torch.autograd.grad(norm(emb(IDS)).square().sum(), params)
+    assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))
+
+
+def test_compiled_callers_run_the_kernels(layers):
+    """torch.compile breaks its graph at the kernels and calls them."""
+    emb, norm = layers.NodeEmbedding(5, 8), layers.LayerNorm(8)
+    step = torch.compile(lambda i: (norm(emb(i) * 2.0) + 1.0).square().sum(), backend="eager")
+    for requires_grad in (True, False):
+        for p in (*emb.parameters(), *norm.parameters()):
+            p.requires_grad_(requires_grad)
+            p.grad = None
+        for _ in range(2):
+            before = layers.kernels.calls
+            loss = step(IDS)
+            assert layers.kernels.calls >= before + 2
+            torch.testing.assert_close(loss, (norm(emb(IDS) * 2.0) + 1.0).square().sum())
+        if requires_grad:
+            loss.backward()
+            got = emb.weight.grad.clone()
+            (want,) = torch.autograd.grad((norm(emb(IDS) * 2.0) + 1.0).square().sum(), emb.weight)
+            torch.testing.assert_close(got, want)
